@@ -92,7 +92,9 @@ def build(force: bool = False, verbose: bool = False, sanitize: bool = False) ->
     host_hdrs = sorted(p for p in CSRC.rglob("*.h")) + sorted(CSRC.rglob("*.hpp"))
 
     hip_flags = [f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-ffast-math",
-                 "-fno-finite-math-only", "-DNDEBUG", f"-I{CSRC}"]
+                 "-fno-finite-math-only", "-DNDEBUG", f"-I{CSRC}",
+                 # no packed fp32 instructions: some of their forms have returned wrong results on this hardware
+                 "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
     host_flags = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall", "-Wno-unused-function",
                   "-Wno-unknown-pragmas", "-Wno-sign-compare",
                   "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DUSE_C10D_GLOO", "-DUSE_C10D_NCCL",
