@@ -555,6 +555,188 @@ std::vector<at::Tensor> linear_wgrad_segments(const std::vector<at::Tensor>& dys
   return {dw, db};
 }
 
+// -------------------------------------------------------- 8-bit floating point --
+// (e4m3 values with a scale byte e + 127 per block of 128; layouts in kernels/pda_kernels.h)
+int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+struct Fp8Pair {
+  at::Tensor q, scale;
+};
+
+// A bf16 / fp32 GPU matrix whose rows are contiguous (any row pitch).
+void check_fp8_source(const at::Tensor& x, const char* name) {
+  TORCH_CHECK(x.is_cuda(), "fp8: ", name, " must live on the GPU");
+  TORCH_CHECK(x.dim() == 2, "fp8: ", name, " must be a matrix, got ", x.dim(), " dimensions");
+  (void)dtype_of(x);
+  TORCH_CHECK(x.numel() == 0 || x.size(1) == 1 || x.stride(1) == 1, "fp8: rows of ", name, " must be contiguous");
+  TORCH_CHECK(x.numel() == 0 || x.size(0) == 1 || x.stride(0) >= x.size(1), "fp8: rows of ", name, " must not overlap");
+  TORCH_CHECK(x.size(0) <= (1 << 22) && x.size(1) <= (1 << 22), "fp8: ", name, " is larger than 2^22 rows or columns");
+}
+
+// Quantises x [R, C] by rows and / or columns, or by tiles (then both layouts share the scales). An output
+// that is not wanted stays undefined. `sums`: fp32 [ceil(R / 128), C] partial column sums (not with tiles).
+void fp8_quantize_into(const at::Tensor& x, bool tiles, Fp8Pair* rows, Fp8Pair* cols, at::Tensor* sums) {
+  const int64_t R = x.size(0), C = x.size(1), Rb = (R + 127) / 128, Cb = (C + 127) / 128;
+  const auto q8 = x.options().dtype(at::kFloat8_e4m3fn), u8 = x.options().dtype(at::kByte);
+  if (rows) {
+    rows->q = at::empty({R, Cb * 128}, q8);
+    rows->scale = at::empty({tiles ? Rb : R, round_up(Cb, 4)}, u8);
+  }
+  if (cols) {
+    cols->q = at::empty({C, Rb * 128}, q8);
+    cols->scale = at::empty({tiles ? Cb : C, round_up(Rb, 4)}, u8);
+  }
+  if (sums) *sums = at::empty({Rb, C}, x.options().dtype(at::kFloat));
+  if (R == 0 || C == 0) return;  // every output is empty
+  auto bytes = [](const at::Tensor& t) { return reinterpret_cast<uint8_t*>(t.data_ptr()); };
+  pda::fp8_quantize(dtype_of(x), x.data_ptr(), R > 1 ? x.stride(0) : C, (int)R, (int)C, tiles, rows ? bytes(rows->q) : nullptr,
+                    rows ? bytes(rows->scale) : nullptr, cols ? bytes(cols->q) : nullptr,
+                    cols ? bytes(cols->scale) : nullptr, sums ? sums->data_ptr<float>() : nullptr, current_stream());
+  check_launch("fp8_quantize");
+}
+
+std::vector<at::Tensor> fp8_quantize(const at::Tensor& x, bool want_rows, bool want_cols, bool tiles) {
+  check_fp8_source(x, "x");
+  TORCH_CHECK(want_rows || want_cols, "fp8_quantize: no output asked for");
+  const c10::DeviceGuard guard(x.device());
+  Fp8Pair rows, cols;
+  fp8_quantize_into(x, tiles, want_rows ? &rows : nullptr, want_cols ? &cols : nullptr, nullptr);
+  std::vector<at::Tensor> out;
+  if (want_rows) out.insert(out.end(), {rows.q, rows.scale});
+  if (want_cols) out.insert(out.end(), {cols.q, cols.scale});
+  return out;
+}
+
+// Checks a quantised operand with `K` values in a row and describes it to the kernel.
+pda::Fp8Operand fp8_operand(const at::Tensor& q, const at::Tensor& scale, bool tiles, int64_t K, const char* name) {
+  TORCH_CHECK(q.is_cuda() && scale.is_cuda() && q.device() == scale.device(), "fp8: ", name, " must live on one GPU");
+  TORCH_CHECK(q.scalar_type() == at::kFloat8_e4m3fn && scale.scalar_type() == at::kByte, "fp8: ", name,
+              " needs float8_e4m3fn values and uint8 scales, got ", q.scalar_type(), " and ", scale.scalar_type());
+  TORCH_CHECK(q.dim() == 2 && scale.dim() == 2 && q.is_contiguous() && scale.is_contiguous(), "fp8: ", name,
+              " needs contiguous matrices");
+  const int64_t Kp = round_up(K, 128), rows = q.size(0);
+  TORCH_CHECK(q.size(1) == Kp, "fp8: ", name, " has rows of ", q.size(1), " values, ", Kp, " expected (", K, " padded to 128)");
+  TORCH_CHECK(scale.size(0) == (tiles ? (rows + 127) / 128 : rows) && scale.size(1) == round_up(Kp / 128, 4), "fp8: ", name,
+              " has scales ", scale.sizes(), ", expected [", tiles ? (rows + 127) / 128 : rows, ", ", round_up(Kp / 128, 4), "]");
+  TORCH_CHECK(rows <= (1 << 22) && Kp <= (1 << 22), "fp8: ", name, " is larger than 2^22 rows or columns");
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0 && reinterpret_cast<uintptr_t>(scale.data_ptr()) % 4 == 0,
+              "fp8: ", name, " must be 16-byte aligned");
+  return pda::Fp8Operand{q.data_ptr(), scale.data_ptr(), Kp, scale.size(1), (int)rows, tiles};
+}
+
+// out[M, N] = (out +) bias + x . w^T; `out` fresh in `dtype` unless given.
+at::Tensor fp8_product(const Fp8Pair& x, bool x_tiles, const Fp8Pair& w, bool w_tiles, int64_t K,
+                       const std::optional<at::Tensor>& bias, at::ScalarType dtype, const std::optional<at::Tensor>& out,
+                       bool accumulate) {
+  const pda::Fp8Operand X = fp8_operand(x.q, x.scale, x_tiles, K, "the left operand");
+  const pda::Fp8Operand W = fp8_operand(w.q, w.scale, w_tiles, K, "the right operand");
+  TORCH_CHECK(x.q.device() == w.q.device(), "fp8_matmul: operands on different devices");
+  const int64_t M = X.rows, N = W.rows;
+  at::Tensor y;
+  if (out.has_value()) {
+    y = *out;
+    TORCH_CHECK(y.device() == x.q.device() && y.is_contiguous() && y.numel() == M * N, "fp8_matmul: out must be a contiguous tensor with ",
+                M * N, " elements on the operands' device");
+  } else {
+    TORCH_CHECK(!accumulate, "fp8_matmul: accumulate needs an out tensor");
+    TORCH_CHECK(dtype == at::kBFloat16 || dtype == at::kFloat, "fp8_matmul: out dtype must be bfloat16 or float32, got ", dtype);
+    y = at::empty({M, N}, x.q.options().dtype(dtype));
+  }
+  const pda::DType out_dtype = dtype_of(y);
+  if (bias.has_value())
+    TORCH_CHECK(bias->device() == x.q.device() && bias->is_contiguous() && bias->numel() == N, "fp8_matmul: bias must be a contiguous tensor with ",
+                N, " elements on the operands' device");
+  const pda::DType bias_dtype = bias.has_value() ? dtype_of(*bias) : pda::kBF16;
+  if (M == 0 || N == 0) return y;
+  if (K == 0) {  // a sum over nothing
+    if (!accumulate) y.zero_();
+    if (bias.has_value()) y.view({M, N}).add_(*bias);
+    return y;
+  }
+  const pda::Fp8GemmPlan plan = pda::fp8_gemm_plan((int)M, (int)N, (int)X.ld, out_dtype);
+  at::Tensor partial;
+  if (plan.slices > 1) partial = at::empty({plan.slices, M, N}, x.q.options().dtype(at::kFloat));
+  pda::fp8_gemm(X, W, (int)X.ld, bias.has_value() ? bias->data_ptr() : nullptr, bias_dtype, y.data_ptr(), out_dtype, accumulate,
+                plan, plan.slices > 1 ? partial.data_ptr<float>() : nullptr, current_stream());
+  check_launch("fp8_gemm");
+  return y;
+}
+
+at::Tensor fp8_matmul(const at::Tensor& xq, const at::Tensor& xs, bool x_tiles, const at::Tensor& wq, const at::Tensor& ws,
+                      bool w_tiles, int64_t K, const std::optional<at::Tensor>& bias, bool out_f32) {
+  TORCH_CHECK(xq.is_cuda(), "fp8_matmul: operands must live on the GPU");
+  const c10::DeviceGuard guard(xq.device());
+  return fp8_product({xq, xs}, x_tiles, {wq, ws}, w_tiles, K, bias, out_f32 ? at::kFloat : at::kBFloat16, std::nullopt, false);
+}
+
+// y = x . w^T + bias with x [M, K] quantised by rows and w [N, K] by tiles. `keep`: also x quantised by
+// columns (from the same read of x), which is all that the weight gradient needs of it.
+std::vector<at::Tensor> fp8_linear_forward(const at::Tensor& x, const at::Tensor& weight, const std::optional<at::Tensor>& bias,
+                                           bool keep) {
+  check_fp8_source(x, "x");
+  check_fp8_source(weight, "weight");
+  TORCH_CHECK(x.scalar_type() == weight.scalar_type() && x.device() == weight.device() && x.size(1) == weight.size(1),
+              "fp8_linear: x ", x.sizes(), " ", x.scalar_type(), " and weight ", weight.sizes(), " ", weight.scalar_type(), " do not match");
+  const c10::DeviceGuard guard(x.device());
+  Fp8Pair xr, xc, wr;
+  fp8_quantize_into(x, false, &xr, keep ? &xc : nullptr, nullptr);
+  fp8_quantize_into(weight, true, &wr, nullptr, nullptr);
+  at::Tensor y = fp8_product(xr, false, wr, true, x.size(1), bias, x.scalar_type(), std::nullopt, false);
+  if (keep) return {y, xc.q, xc.scale};
+  return {y};
+}
+
+// Gradients of that: dx = dy . w (dy by rows, w by tiles), dw = dy^T . x (both by columns), db = column sums of
+// dy before quantisation. xq / xs: x by columns (fp8_linear_forward's `keep`), or `x` itself, quantised here.
+std::vector<at::Tensor> fp8_linear_backward(const at::Tensor& dy, const at::Tensor& weight, const std::optional<at::Tensor>& x,
+                                            const std::optional<at::Tensor>& xq, const std::optional<at::Tensor>& xs, bool want_x,
+                                            bool want_w, bool want_b, const std::optional<at::Tensor>& w_out, bool w_accumulate,
+                                            const std::optional<at::Tensor>& b_out, bool b_accumulate) {
+  check_fp8_source(dy, "dy");
+  check_fp8_source(weight, "weight");
+  const int64_t M = dy.size(0), N = dy.size(1), K = weight.size(1);
+  TORCH_CHECK(dy.scalar_type() == weight.scalar_type() && dy.device() == weight.device() && weight.size(0) == N,
+              "fp8_linear backward: dy ", dy.sizes(), " ", dy.scalar_type(), " and weight ", weight.sizes(), " ", weight.scalar_type(), " do not match");
+  const c10::DeviceGuard guard(dy.device());
+  Fp8Pair gr, gc, wc, xc;
+  at::Tensor sums, dx, dw, db;
+  if (want_x || want_w || want_b)  // (the bias gradient alone still needs the pass: rows are the cheaper by-product)
+    fp8_quantize_into(dy, false, want_x || !want_w ? &gr : nullptr, want_w ? &gc : nullptr, want_b ? &sums : nullptr);
+  if (want_x) {
+    fp8_quantize_into(weight, true, nullptr, &wc, nullptr);
+    dx = fp8_product(gr, false, wc, true, N, std::nullopt, dy.scalar_type(), std::nullopt, false);
+  }
+  if (want_w) {
+    if (x.has_value()) {
+      check_fp8_source(*x, "x");
+      TORCH_CHECK(x->size(0) == M && x->size(1) == K && x->scalar_type() == dy.scalar_type() && x->device() == dy.device(),
+                  "fp8_linear backward: x ", x->sizes(), " does not match dy ", dy.sizes());
+      fp8_quantize_into(*x, false, nullptr, &xc, nullptr);
+    } else {
+      TORCH_CHECK(xq.has_value() && xs.has_value(), "fp8_linear backward: the weight gradient needs x");
+      xc = {*xq, *xs};
+    }
+    dw = fp8_product(gc, false, xc, false, M, std::nullopt, dy.scalar_type(), w_out, w_accumulate);
+    if (!w_out.has_value()) dw = dw.view({N, K});
+  }
+  if (want_b) {
+    if (b_out.has_value()) {
+      db = *b_out;
+      TORCH_CHECK(db.device() == dy.device() && db.is_contiguous() && db.numel() == N,
+                  "fp8_linear backward: bias_out must be a contiguous tensor with ", N, " elements");
+    } else {
+      TORCH_CHECK(!b_accumulate, "fp8_linear backward: accumulating the bias gradient needs its tensor");
+      db = at::empty({N}, dy.options());
+    }
+    if (N > 0) {
+      pda::fp8_fold_column_sums(M > 0 ? sums.data_ptr<float>() : nullptr, (int)((M + 127) / 128), (int)N, dtype_of(db), db.data_ptr(),
+                                b_accumulate, current_stream());
+      check_launch("fp8_fold_column_sums");
+    }
+  }
+  return {dx, dw, db};
+}
+
 }  // namespace
 
 // ------------------------------------------------------- fused-epilogue GEMM --
@@ -725,6 +907,13 @@ void bind_ops(py::module_& m) {
         py::arg("eps"), py::arg("weight_decay"), py::arg("step"), py::arg("grad_scale"),
         py::arg("zero_grad"), py::arg("dynamic") = py::none());
   m.def("accumulate_bf16_into_f32", &accumulate_bf16_into_f32);
+  m.def("fp8_quantize", &fp8_quantize, py::arg("x"), py::arg("rows"), py::arg("columns"), py::arg("tiles"));
+  m.def("fp8_matmul", &fp8_matmul, py::arg("xq"), py::arg("xs"), py::arg("x_tiles"), py::arg("wq"), py::arg("ws"),
+        py::arg("w_tiles"), py::arg("K"), py::arg("bias"), py::arg("out_f32"));
+  m.def("fp8_linear_forward", &fp8_linear_forward, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("keep"));
+  m.def("fp8_linear_backward", &fp8_linear_backward, py::arg("dy"), py::arg("weight"), py::arg("x"), py::arg("xq"), py::arg("xs"),
+        py::arg("want_x"), py::arg("want_w"), py::arg("want_b"), py::arg("w_out"), py::arg("w_accumulate"), py::arg("b_out"),
+        py::arg("b_accumulate"));
   m.def("attention_forward", &attention_forward, py::arg("qkv"), py::arg("num_heads"),
         py::arg("softmax_scale"), py::arg("dropout_p") = 0.0, py::arg("seed") = 0);
   m.def("attention_backward", &attention_backward, py::arg("qkv"), py::arg("out"), py::arg("dout"),

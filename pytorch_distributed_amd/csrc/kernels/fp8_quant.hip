@@ -1,0 +1,291 @@
+// Block quantisation to 8-bit floating point (OCP e4m3) for gfx950.
+//
+// A block of 128 values shares a power-of-two scale 2^e with
+//     e = min { integer >= -127 : max|x| <= 448 * 2^e },     q = e4m3(x / 2^e), ties to even,
+// stored as the byte e + 127 (the E8M0 form the block-scaled matrix instruction takes). Dividing by a
+// power of two is exact, so the rounding to e4m3 is the only error: at most half a step, 2^-4 of a
+// normal value. With max|x| = m 2^k (1 <= m < 2) and 448 = 1.75 * 2^8, e = k - 8, plus one when
+// m > 1.75: read off the float's bits, no logarithm. An infinity or a NaN takes no part in its block's
+// maximum and becomes the e4m3 NaN (0x7f / 0xff), so a product with it is NaN where bf16 would be.
+//
+// Three block shapes, any combination of the two outputs in ONE pass over x [R, C]:
+//   rows      1 x 128 along C:  q [R, Cp],  scale [R, Sc]       (contraction over C)
+//   columns   128 x 1 along R:  qt [C, Rp], scale [C, Sr]       (transposed: contraction over R)
+//   tiles     128 x 128, one scale, both layouts                (weights: both contractions)
+// Cp / Rp are C / R rounded up to 128 (padding: zeros), Sc / Sr the block counts rounded up to 4
+// (padding: zero bytes). The column sums of x (a bias gradient) can ride along: fp32 partial sums per
+// 128-row block, folded in block order by fp8_fold_column_sums.
+//
+// What bounds it: memory. A workgroup owns a 128 x 128 tile held in registers (8 rows x 8 columns per
+// thread), so x is read once for both layouts; the transposed bytes pass through a swizzled 16 KiB LDS
+// tile and leave as whole 128-byte lines.
+#include "common.h"
+#include "pda_kernels.h"
+
+namespace pda {
+namespace {
+
+constexpr int kBlock = 128;
+constexpr int kThreads = 256;
+constexpr float kInf = __builtin_inff();
+
+// Scale byte of a block with largest finite magnitude `amax` (>= 0), from the float's exponent and
+// mantissa. Subnormal magnitudes are far below 448 * 2^-127: byte 0.
+__device__ __forceinline__ uint32_t scale_byte(float amax) {
+  const uint32_t u = __float_as_uint(amax);
+  const int e = int(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);  // biased exponent - 8 = (e + 127)
+  return uint32_t(max(e, 0));
+}
+
+// 2^-(byte - 127). Bytes run from 0 to 248 (max float: 2^127 * 2 / 448), so the result is a normal float.
+__device__ __forceinline__ float inverse_scale(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
+
+__device__ __forceinline__ uint32_t pack_fp8x4(float a, float b, float c, float d) {
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true));
+}
+
+// |x| of the finite values, 0 for the others.
+__device__ __forceinline__ float finite_abs(float x) {
+  const float a = __builtin_fabsf(x);
+  return a < kInf ? a : 0.f;
+}
+
+// Eight values of one row starting at column c (c % 8 == 0); columns >= C and rows >= R read as zeros.
+template <typename T, bool kVec>
+__device__ __forceinline__ void load8(const T* __restrict__ x, int64_t ld, int R, int C, int row, int c, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = 0.f;
+  if (row >= R || c >= C) return;
+  const T* p = x + int64_t(row) * ld + c;
+  if (kVec && c + 8 <= C) {
+    if constexpr (sizeof(T) == 2) {
+      VecIO<T>::load(p, v);
+    } else {
+      float a[4], b[4];
+      VecIO<T>::load(p, a);
+      VecIO<T>::load(p + 4, b);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (c + i < C) v[i] = VecIO<T>::load1(p + i);
+}
+
+// Thread (g = tid / 16, j = tid % 16) holds rows 8 g .. 8 g + 7 and columns 8 j .. 8 j + 7 of the tile.
+template <typename T, bool kVec, bool kRows, bool kCols, bool kTiles, bool kSums>
+__global__ __launch_bounds__(kThreads) void quantize_kernel(const T* __restrict__ x, int64_t ld, int R, int C,
+                                                            uint8_t* __restrict__ q, uint8_t* __restrict__ s,
+                                                            uint8_t* __restrict__ qt, uint8_t* __restrict__ st,
+                                                            float* __restrict__ sums) {
+  __shared__ __attribute__((aligned(16))) uint8_t tile[kCols ? kBlock * kBlock : 16];
+  __shared__ float red[4][kBlock];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int g = tid >> 4, j = tid & 15;
+  const int cb = blockIdx.x, rb = blockIdx.y;
+  const int n_cb = (C + kBlock - 1) / kBlock, n_rb = (R + kBlock - 1) / kBlock;
+  const int row0 = rb * kBlock + 8 * g, col0 = cb * kBlock + 8 * j;
+
+  float v[8][8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) load8<T, kVec>(x, ld, R, C, row0 + i, col0, v[i]);
+
+  float tile_inv = 1.f;
+  uint32_t tile_byte = 0;
+  if constexpr (kTiles) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) m = fmaxf(m, finite_abs(v[i][k]));
+    m = block_max<kThreads>(m, &red[0][0]);
+    tile_byte = scale_byte(m);
+    tile_inv = inverse_scale(tile_byte);
+    // one byte per tile in each orientation; the last tile of a row of tiles also clears the padding
+    if (tid == 0) {
+      if (kRows) {
+        const int pitch = (n_cb + 3) & ~3;
+        s[int64_t(rb) * pitch + cb] = uint8_t(tile_byte);
+        if (cb == n_cb - 1)
+          for (int k = n_cb; k < pitch; ++k) s[int64_t(rb) * pitch + k] = 0;
+      }
+      if (kCols) {
+        const int pitch = (n_rb + 3) & ~3;
+        st[int64_t(cb) * pitch + rb] = uint8_t(tile_byte);
+        if (rb == n_rb - 1)
+          for (int k = n_rb; k < pitch; ++k) st[int64_t(cb) * pitch + k] = 0;
+      }
+    }
+  }
+
+  if constexpr (kRows) {
+    const int64_t Cp = int64_t(n_cb) * kBlock;
+    const int pitch = (n_cb + 3) & ~3;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int row = row0 + i;
+      float inv = tile_inv;
+      if constexpr (!kTiles) {
+        float m = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) m = fmaxf(m, finite_abs(v[i][k]));
+#pragma unroll
+        for (int off = 8; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+        const uint32_t byte = scale_byte(m);
+        inv = inverse_scale(byte);
+        if (row < R && j == 0) {
+          s[int64_t(row) * pitch + cb] = uint8_t(byte);
+          if (cb == n_cb - 1)
+            for (int k = n_cb; k < pitch; ++k) s[int64_t(row) * pitch + k] = 0;
+        }
+      }
+      if (row < R) {
+        u32x2 w = {pack_fp8x4(v[i][0] * inv, v[i][1] * inv, v[i][2] * inv, v[i][3] * inv),
+                   pack_fp8x4(v[i][4] * inv, v[i][5] * inv, v[i][6] * inv, v[i][7] * inv)};
+        *reinterpret_cast<u32x2*>(q + int64_t(row) * Cp + col0) = w;
+      }
+    }
+  }
+
+  if constexpr (kSums) {  // column sums of this 128-row block: rows in a thread, row groups in a wave, waves in order
+    float sum[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      sum[k] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[k] += v[i][k];
+      sum[k] += __shfl_xor(sum[k], 16, 64);
+      sum[k] += __shfl_xor(sum[k], 32, 64);
+    }
+    if (lane < 16)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) red[wave][8 * j + k] = sum[k];
+    __syncthreads();
+    if (tid < kBlock && cb * kBlock + tid < C)
+      sums[int64_t(rb) * C + cb * kBlock + tid] = (red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid]);
+    __syncthreads();
+  }
+
+  if constexpr (kCols) {
+    float inv[8];
+    if constexpr (kTiles) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) inv[k] = tile_inv;
+    } else {
+      float m[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        m[k] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m[k] = fmaxf(m[k], finite_abs(v[i][k]));
+        m[k] = fmaxf(m[k], __shfl_xor(m[k], 16, 64));
+        m[k] = fmaxf(m[k], __shfl_xor(m[k], 32, 64));
+      }
+      if (lane < 16)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) red[wave][8 * j + k] = m[k];
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int c = 8 * j + k;
+        const uint32_t byte = scale_byte(fmaxf(fmaxf(red[0][c], red[1][c]), fmaxf(red[2][c], red[3][c])));
+        inv[k] = inverse_scale(byte);
+        if (g == 0 && col0 + k < C) {
+          const int pitch = (n_rb + 3) & ~3;
+          uint8_t* dst = st + int64_t(col0 + k) * pitch;
+          dst[rb] = uint8_t(byte);
+          if (rb == n_rb - 1)
+            for (int b = n_rb; b < pitch; ++b) dst[b] = 0;
+        }
+      }
+    }
+    // Column c of the tile is a 128-byte LDS row; its 16-byte chunks are permuted by the column group j
+    // (the lanes of a store share the column within their group), so 8 column groups take 8 chunks.
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      u32x2 w = {pack_fp8x4(v[0][k] * inv[k], v[1][k] * inv[k], v[2][k] * inv[k], v[3][k] * inv[k]),
+                 pack_fp8x4(v[4][k] * inv[k], v[5][k] * inv[k], v[6][k] * inv[k], v[7][k] * inv[k])};
+      const int chunk = (g >> 1) ^ (j & 7);
+      *reinterpret_cast<u32x2*>(&tile[(8 * j + k) * kBlock + chunk * 16 + (g & 1) * 8]) = w;
+    }
+    __syncthreads();
+    const int64_t Rp = int64_t(n_rb) * kBlock;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = i * 32 + (tid >> 3), chunk = tid & 7;  // 8 lanes write one 128-byte line
+      const u32x4 w = *reinterpret_cast<const u32x4*>(&tile[c * kBlock + (chunk ^ ((c >> 3) & 7)) * 16]);
+      const int col = cb * kBlock + c;
+      if (col < C) *reinterpret_cast<u32x4*>(qt + int64_t(col) * Rp + int64_t(rb) * kBlock + chunk * 16) = w;
+    }
+  }
+}
+
+template <typename Out>
+__global__ __launch_bounds__(kThreads) void fold_column_sums_kernel(const float* __restrict__ sums, int n_rb, int C,
+                                                                    Out* __restrict__ out, bool accumulate) {
+  // 64 columns per workgroup; wave w adds the blocks w, w + 4, ... and the four sums meet in LDS.
+  __shared__ float red[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int c = blockIdx.x * 64 + lane;
+  float a = 0.f;
+  if (c < C)
+    for (int b = wave; b < n_rb; b += 4) a += sums[int64_t(b) * C + c];
+  red[wave][lane] = a;
+  __syncthreads();
+  if (wave == 0 && c < C) {
+    a = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+    if (accumulate) a += VecIO<Out>::load1(out + c);
+    VecIO<Out>::store1(out + c, a);
+  }
+}
+
+template <typename T, bool kVec>
+void launch_quantize(const T* x, int64_t ld, int R, int C, bool tiles, uint8_t* q, uint8_t* s, uint8_t* qt, uint8_t* st,
+                     float* sums, hipStream_t stream) {
+  const dim3 grid((unsigned)ceil_div(C, kBlock), (unsigned)ceil_div(R, kBlock)), block(kThreads);
+  auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, block, 0, stream, x, ld, R, C, q, s, qt, st, sums); };
+  if (tiles) {
+    if (q && qt) go(quantize_kernel<T, kVec, true, true, true, false>);
+    else if (q) go(quantize_kernel<T, kVec, true, false, true, false>);
+    else go(quantize_kernel<T, kVec, false, true, true, false>);
+  } else if (sums) {
+    if (q && qt) go(quantize_kernel<T, kVec, true, true, false, true>);
+    else if (q) go(quantize_kernel<T, kVec, true, false, false, true>);
+    else go(quantize_kernel<T, kVec, false, true, false, true>);
+  } else {
+    if (q && qt) go(quantize_kernel<T, kVec, true, true, false, false>);
+    else if (q) go(quantize_kernel<T, kVec, true, false, false, false>);
+    else go(quantize_kernel<T, kVec, false, true, false, false>);
+  }
+}
+
+}  // namespace
+
+void fp8_quantize(DType dtype, const void* x, int64_t ld, int R, int C, bool tiles, uint8_t* q, uint8_t* scale,
+                  uint8_t* qt, uint8_t* scale_t, float* column_sums, hipStream_t stream) {
+  const int size = dtype == kBF16 ? 2 : 4;
+  const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (ld * size) % 16 == 0;
+  if (dtype == kBF16) {
+    const auto* p = (const bf16_raw*)x;
+    if (vec) launch_quantize<bf16_raw, true>(p, ld, R, C, tiles, q, scale, qt, scale_t, column_sums, stream);
+    else launch_quantize<bf16_raw, false>(p, ld, R, C, tiles, q, scale, qt, scale_t, column_sums, stream);
+  } else {
+    const auto* p = (const float*)x;
+    if (vec) launch_quantize<float, true>(p, ld, R, C, tiles, q, scale, qt, scale_t, column_sums, stream);
+    else launch_quantize<float, false>(p, ld, R, C, tiles, q, scale, qt, scale_t, column_sums, stream);
+  }
+}
+
+void fp8_fold_column_sums(const float* sums, int n_blocks, int C, DType out_dtype, void* out, bool accumulate,
+                          hipStream_t stream) {
+  const dim3 grid((unsigned)ceil_div(C, 64)), block(kThreads);
+  if (out_dtype == kBF16)
+    hipLaunchKernelGGL(fold_column_sums_kernel<bf16_raw>, grid, block, 0, stream, sums, n_blocks, C, (bf16_raw*)out, accumulate);
+  else
+    hipLaunchKernelGGL(fold_column_sums_kernel<float>, grid, block, 0, stream, sums, n_blocks, C, (float*)out, accumulate);
+}
+
+}  // namespace pda

@@ -152,6 +152,35 @@ bool gemm_fused_supported(int M, int N, int K);
 void gemm_fused(const void* X, int64_t ldx, const void* W, int64_t ldw, const void* bias, void* out, int64_t ldo, void* aux,
                 int64_t ldaux, int M, int N, int K, int epilogue, hipStream_t stream);
 
+// ------------------------------------------------------- 8-bit floating point --
+// Block quantisation of x [R, C] (row pitch ld elements, bf16 / fp32) to e4m3 with a scale byte e + 127 per
+// block of 128: q [R, Cp] + scale [R, Sc] (blocks along rows), qt [C, Rp] + scale_t [C, Sr] (blocks along
+// columns, transposed), or with `tiles` one scale per 128 x 128 tile (scale [ceil(R/128), Sc], scale_t
+// [ceil(C/128), Sr]). Cp / Rp: rounded up to 128, Sc / Sr: block counts rounded up to 4; all padding is
+// zeroed. Either output pair may be null. column_sums (without tiles): fp32 [ceil(R/128), C] partial sums of
+// x, folded in order by fp8_fold_column_sums into out [C].
+void fp8_quantize(DType dtype, const void* x, int64_t ld, int R, int C, bool tiles, uint8_t* q, uint8_t* scale,
+                  uint8_t* qt, uint8_t* scale_t, float* column_sums, hipStream_t stream);
+void fp8_fold_column_sums(const float* sums, int n_blocks, int C, DType out_dtype, void* out, bool accumulate,
+                          hipStream_t stream);
+// out[M, N] = (out +) bias + x . w^T for such operands: `rows` rows of ld bytes (K of them read, K % 128 == 0),
+// scales at row (or row / 128 with `tiles`), ld_scale bytes a row (a multiple of 4, at least K / 128). out and
+// the bias are contiguous. fp8_gemm_plan chooses the tile and how often the contraction is cut; more than one
+// slice needs `partial`, fp32 [slices][M][N].
+struct Fp8Operand {
+  const void* q;
+  const void* scale;
+  int64_t ld, ld_scale;
+  int rows;
+  bool tiles;
+};
+struct Fp8GemmPlan {
+  int tile, slices, steps_per_slice;
+};
+Fp8GemmPlan fp8_gemm_plan(int M, int N, int K, DType out_dtype);
+void fp8_gemm(const Fp8Operand& x, const Fp8Operand& w, int K, const void* bias, DType bias_dtype, void* out,
+              DType out_dtype, bool accumulate, const Fp8GemmPlan& plan, float* partial, hipStream_t stream);
+
 // ----------------------------------------------------------------- Embedding --
 // out[n, :] = wte[ids[n], :] (+ wpe[n mod T, :] when wpe != nullptr). d % (16 / sizeof(T)) == 0.
 void embedding_forward(DType dtype, const int64_t* ids, const void* wte, const void* wpe, void* out, int64_t n_tokens,
