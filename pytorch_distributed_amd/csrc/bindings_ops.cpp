@@ -9,6 +9,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <optional>
 #include <vector>
 
@@ -350,6 +351,65 @@ at::Tensor attention_backward(const at::Tensor& qkv, const at::Tensor& out, cons
                           delta.data_ptr<float>(), dqkv.data_ptr(), (int)B, (int)T, (int)num_heads,
                           (int)D, (float)softmax_scale, (float)dropout_p, seed, current_stream());
   check_launch("attention_backward");
+  return dqkv;
+}
+
+// Checks of both window-attention passes; returns {B, T, D} and clamps window and sinks to the length.
+struct WindowShape {
+  int64_t B, T, H, D, window, sinks;
+};
+WindowShape check_window(const at::Tensor& qkv, int64_t num_heads, int64_t window, int64_t sinks, double dropout_p) {
+  check_gpu(qkv, "qkv");
+  TORCH_CHECK(qkv.scalar_type() == at::kBFloat16, "window attention: bf16 only");
+  TORCH_CHECK(qkv.dim() == 3, "window attention: qkv must be [B, T, 3*H*D]");
+  TORCH_CHECK(num_heads >= 1 && qkv.size(2) % (3 * num_heads) == 0, "window attention: bad qkv width");
+  TORCH_CHECK(window >= 1, "window attention: window must be at least 1, got ", window);
+  TORCH_CHECK(sinks >= 0, "window attention: sinks must not be negative, got ", sinks);
+  TORCH_CHECK(dropout_p >= 0.0 && dropout_p < 1.0, "window attention: dropout_p must be in [0, 1)");
+  WindowShape w{qkv.size(0), qkv.size(1), num_heads, qkv.size(2) / (3 * num_heads), window, sinks};
+  TORCH_CHECK(w.D == 64 || w.D == 128, "window attention: head_dim must be 64 or 128, got ", w.D);
+  TORCH_CHECK(w.B >= 1 && w.T >= 1, "window attention: empty input");
+  TORCH_CHECK(w.T <= (1 << 30) && (w.T / 128 + 1) * w.B * w.H < (int64_t(1) << 31) && 64 * qkv.size(2) * 2 < (int64_t(1) << 31),
+              "window attention: sizes exceed the kernels' 32-bit indices");
+  w.window = std::min(window, w.T);
+  w.sinks = std::min(sinks, w.T);
+  return w;
+}
+
+std::vector<at::Tensor> window_attention_forward(const at::Tensor& qkv, int64_t num_heads, int64_t window, int64_t sinks,
+                                                 double softmax_scale, double dropout_p, uint64_t seed) {
+  const WindowShape w = check_window(qkv, num_heads, window, sinks, dropout_p);
+  const c10::DeviceGuard guard(qkv.device());
+  at::Tensor out = at::empty({w.B, w.T, w.H * w.D}, qkv.options());
+  at::Tensor lse = at::empty({w.B, w.H, w.T}, qkv.options().dtype(at::kFloat));
+  pda::window_attention_forward(qkv.data_ptr(), out.data_ptr(), lse.data_ptr<float>(), (int)w.B, (int)w.T, (int)w.H, (int)w.D,
+                                (int)w.window, (int)w.sinks, (float)softmax_scale, (float)dropout_p, seed, current_stream());
+  check_launch("window_attention_forward");
+  return {out, lse};
+}
+
+at::Tensor window_attention_backward(const at::Tensor& qkv, const at::Tensor& out, const at::Tensor& dout, const at::Tensor& lse,
+                                     int64_t num_heads, int64_t window, int64_t sinks, double softmax_scale, double dropout_p,
+                                     uint64_t seed) {
+  const WindowShape w = check_window(qkv, num_heads, window, sinks, dropout_p);
+  check_gpu(out, "out");
+  check_gpu(dout, "dout");
+  check_gpu(lse, "lse");
+  TORCH_CHECK(out.scalar_type() == at::kBFloat16 && dout.scalar_type() == at::kBFloat16 && lse.scalar_type() == at::kFloat,
+              "window attention backward: dtype mismatch");
+  TORCH_CHECK(out.numel() == w.B * w.T * w.H * w.D && dout.numel() == out.numel() && lse.numel() == w.B * w.H * w.T,
+              "window attention backward: shape mismatch");
+  TORCH_CHECK(out.device() == qkv.device() && dout.device() == qkv.device() && lse.device() == qkv.device(),
+              "window attention backward: tensors on different devices");
+  const c10::DeviceGuard guard(qkv.device());
+  at::Tensor dqkv = at::empty_like(qkv);
+  at::Tensor delta = at::empty_like(lse);
+  const size_t bytes = pda::window_attention_backward_workspace_bytes((int)w.B, (int)w.T, (int)w.H, (int)w.D, (int)w.window, (int)w.sinks);
+  at::Tensor workspace = at::empty({(int64_t)bytes}, qkv.options().dtype(at::kByte));
+  pda::window_attention_backward(qkv.data_ptr(), out.data_ptr(), dout.data_ptr(), lse.data_ptr<float>(), delta.data_ptr<float>(),
+                                 dqkv.data_ptr(), bytes ? workspace.data_ptr() : nullptr, (int)w.B, (int)w.T, (int)w.H, (int)w.D,
+                                 (int)w.window, (int)w.sinks, (float)softmax_scale, (float)dropout_p, seed, current_stream());
+  check_launch("window_attention_backward");
   return dqkv;
 }
 
@@ -919,6 +979,10 @@ void bind_ops(py::module_& m) {
   m.def("attention_backward", &attention_backward, py::arg("qkv"), py::arg("out"), py::arg("dout"),
         py::arg("lse"), py::arg("num_heads"), py::arg("softmax_scale"), py::arg("dropout_p") = 0.0,
         py::arg("seed") = 0);
+  m.def("window_attention_forward", &window_attention_forward, py::arg("qkv"), py::arg("num_heads"), py::arg("window"),
+        py::arg("sinks"), py::arg("softmax_scale"), py::arg("dropout_p"), py::arg("seed"));
+  m.def("window_attention_backward", &window_attention_backward, py::arg("qkv"), py::arg("out"), py::arg("dout"), py::arg("lse"),
+        py::arg("num_heads"), py::arg("window"), py::arg("sinks"), py::arg("softmax_scale"), py::arg("dropout_p"), py::arg("seed"));
   m.def("attention_dropout_mask", &attention_dropout_mask, py::arg("B"), py::arg("H"), py::arg("T"),
         py::arg("dropout_p"), py::arg("seed"), py::arg("device"));
 }

@@ -101,6 +101,16 @@ void attention_backward(const void* qkv, const void* out, const void* dout, cons
 // keep[B*H][T][T] (bytes): 1 where the dropout mask of (dropout_p, seed) keeps the probability.
 void attention_dropout_mask(uint8_t* keep, int B, int T, int H, float dropout_p, uint64_t seed, hipStream_t stream);
 
+// The same inside a sliding window with sinks: query t sees keys s <= t with t - s < window or s < sinks
+// (1 <= window <= T, 0 <= sinks <= T). lse is in log2 units and goes back to the backward as it came. The
+// backward's workspace may be null where its size is 0.
+void window_attention_forward(const void* qkv, void* out, float* lse, int B, int T, int H, int D, int window, int sinks,
+                              float softmax_scale, float dropout_p, uint64_t seed, hipStream_t stream);
+size_t window_attention_backward_workspace_bytes(int B, int T, int H, int D, int window, int sinks);
+void window_attention_backward(const void* qkv, const void* out, const void* dout, const float* lse, float* delta,
+                               void* dqkv, void* workspace, int B, int T, int H, int D, int window, int sinks,
+                               float softmax_scale, float dropout_p, uint64_t seed, hipStream_t stream);
+
 // ------------------------------------------------------------------- Rotary --
 // Rotates the Q and K thirds of a packed [B, T, 3, H, D] activation (rotate-half pairing) by
 // the angles of the fp32 tables cos / sin [>= T, D/2]; `inverse` rotates back (the backward).

@@ -35,15 +35,26 @@ import torch.nn.functional as F
 from .. import _ext
 
 
+def visible_mask(T: int, window: int | None = None, sinks: int = 0, device=None) -> torch.Tensor:
+    """``[T, T]`` bool: may query t (row) see key s (column)? Causal, and with a ``window`` only where
+    ``t - s < window`` or ``s < sinks``."""
+    mask = torch.ones(T, T, dtype=torch.bool, device=device).tril()
+    if window is not None:
+        near = torch.ones(T, T, dtype=torch.bool, device=device).triu(1 - min(window, T))
+        near[:, :sinks] = True
+        mask &= near
+    return mask
+
+
 def attention_reference(qkv: torch.Tensor, num_heads: int, scale: float | None = None,
                         dropout_p: float = 0.0, training: bool = False, keep_mask=None,
-                        keep_scale: float | None = None) -> torch.Tensor:
+                        keep_scale: float | None = None, window: int | None = None, sinks: int = 0) -> torch.Tensor:
     B, T, three_hd = qkv.shape
     D = three_hd // (3 * num_heads)
     scale = 1.0 / math.sqrt(D) if scale is None else scale
     q, k, v = qkv.float().view(B, T, 3, num_heads, D).permute(2, 0, 3, 1, 4)  # each [B, H, T, D]
     scores = torch.matmul(q, k.transpose(-2, -1)) * scale
-    mask = torch.ones(T, T, dtype=torch.bool, device=qkv.device).tril()
+    mask = visible_mask(T, window, sinks, qkv.device)
     scores = scores.masked_fill(~mask, float("-inf"))
     probs = torch.softmax(scores, dim=-1)
     if keep_mask is not None:  # explicit mask [B, H, T, T] (the kernels' mask in the parity tests)
@@ -110,3 +121,64 @@ def causal_attention(qkv: torch.Tensor, num_heads: int, scale: float | None = No
     if want_dropout or qkv.is_cuda:  # CPU with dropout, or the forced-reference oracle mode on a GPU
         return attention_reference(qkv, num_heads, scale, dropout_p, training)
     return attention_sdpa(qkv, num_heads, scale)
+
+
+def _packed(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous and on a 16-byte boundary, as the kernels' vector loads need it."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+class _WindowAttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, qkv, num_heads, window, sinks, scale, dropout_p, seed):
+        qkv = _packed(qkv)
+        ctx.args = (num_heads, window, sinks, scale, dropout_p, seed)
+        out, lse = _ext.require().window_attention_forward(qkv, *ctx.args)
+        ctx.save_for_backward(qkv, out, lse)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        qkv, out, lse = ctx.saved_tensors
+        dqkv = _ext.require().window_attention_backward(qkv, out, _packed(dout), lse, *ctx.args)
+        return (dqkv,) + (None,) * 6
+
+
+def window_attention(qkv: torch.Tensor, num_heads: int, window: int, sinks: int = 0, scale: float | None = None,
+                     dropout_p: float = 0.0, training: bool = False, seed: int | None = None) -> torch.Tensor:
+    """:func:`causal_attention` inside a sliding window: query t sees the ``window`` keys ``t - window + 1 .. t``
+    (itself included, so ``window >= 1``) and the first ``sinks`` keys of the sequence, which stay visible however
+    far behind they are. Time and memory grow with ``T * window``; a window of T or more is causal attention.
+
+    Layout, dtypes, head sizes, scale and dropout as for :func:`causal_attention` (the same dropout mask for the
+    same seed); on the GPU ``csrc/kernels/attention_window.hip``. A NaN or infinity in a key or value reaches
+    the queries that see it, and may reach others whose tile of 64 keys holds it (as in a plain product of
+    probabilities and values, where a masked probability of zero times an infinity is NaN)."""
+    if qkv.dim() != 3 or num_heads < 1 or qkv.shape[-1] % (3 * num_heads) != 0:
+        raise ValueError(f"window_attention: qkv {tuple(qkv.shape)} is not [B, T, 3 * {num_heads} * head size]")
+    window, sinks = int(window), int(sinks)
+    if window < 1 or sinks < 0:
+        raise ValueError(f"window_attention: window must be at least 1 and sinks at least 0, got {window} and {sinks}")
+    B, T, width = qkv.shape
+    D = width // (3 * num_heads)
+    window, sinks = min(window, max(T, 1)), min(sinks, T)
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    p = float(dropout_p) if training else 0.0
+    if not 0.0 <= p < 1.0:
+        raise ValueError(f"window_attention: dropout_p must be in [0, 1), got {p}")
+    if not _ext.use_hip(qkv):
+        return attention_reference(qkv, num_heads, scale, p, training, window=window, sinks=sinks)
+    if D not in (64, 128) or qkv.dtype not in (torch.bfloat16, torch.float32):
+        raise NotImplementedError(f"window_attention on the GPU: head size {D} / dtype {qkv.dtype} has no kernel "
+                                  "(head sizes 64 and 128; bf16, or fp32 computed through bf16 MFMA inputs)")
+    if scale <= 0.0:
+        raise ValueError(f"window_attention: the kernels take a positive scale, got {scale}")
+    if B * T == 0:
+        return qkv[..., : width // 3] * 0
+    if qkv.dtype == torch.float32:  # fp32 storage: bf16 MFMA inputs, fp32 accumulation, widened result
+        return window_attention(qkv.to(torch.bfloat16), num_heads, window, sinks, scale, p, training, seed).to(torch.float32)
+    if p > 0.0:
+        seed = _draw_seed() if seed is None else int(seed)
+    return _WindowAttentionFn.apply(qkv, num_heads, window, sinks, scale, p, seed if p > 0.0 else 0)
