@@ -376,6 +376,12 @@ WindowShape check_window(const at::Tensor& qkv, int64_t num_heads, int64_t windo
   return w;
 }
 
+// Contiguous and on a 16-byte boundary, as vector loads need it.
+at::Tensor packed16(const at::Tensor& t) {
+  const at::Tensor c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
+}
+
 std::vector<at::Tensor> window_attention_forward(const at::Tensor& qkv, int64_t num_heads, int64_t window, int64_t sinks,
                                                  double softmax_scale, double dropout_p, uint64_t seed) {
   const WindowShape w = check_window(qkv, num_heads, window, sinks, dropout_p);
@@ -411,6 +417,33 @@ at::Tensor window_attention_backward(const at::Tensor& qkv, const at::Tensor& ou
                                  (int)w.window, (int)w.sinks, (float)softmax_scale, (float)dropout_p, seed, current_stream());
   check_launch("window_attention_backward");
   return dqkv;
+}
+
+struct WindowAttentionFn : public torch::autograd::Function<WindowAttentionFn> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& qkv, int64_t num_heads, int64_t window,
+                            int64_t sinks, double softmax_scale, double dropout_p, int64_t seed) {
+    const at::Tensor packed = packed16(qkv);
+    auto got = window_attention_forward(packed, num_heads, window, sinks, softmax_scale, dropout_p, (uint64_t)seed);
+    ctx->save_for_backward({packed, got[0], got[1]});
+    auto& d = ctx->saved_data;
+    d["args"] = std::vector<int64_t>{num_heads, window, sinks, seed};
+    d["floats"] = std::vector<double>{softmax_scale, dropout_p};
+    return got[0];
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "window_attention has no second derivative (create_graph=True)");
+    const auto saved = ctx->get_saved_variables();
+    const auto i = ctx->saved_data["args"].toIntVector();
+    const auto f = ctx->saved_data["floats"].toDoubleVector();
+    at::Tensor dqkv = window_attention_backward(saved[0], saved[1], packed16(grads[0]), saved[2], i[0], i[1], i[2], f[0], f[1], (uint64_t)i[3]);
+    const at::Tensor none;
+    return {dqkv, none, none, none, none, none, none};
+  }
+};
+
+at::Tensor window_attention(const at::Tensor& qkv, int64_t num_heads, int64_t window, int64_t sinks, double softmax_scale,
+                            double dropout_p, int64_t seed) {
+  return WindowAttentionFn::apply(qkv, num_heads, window, sinks, softmax_scale, dropout_p, seed);
 }
 
 // keep[B, H, T, T] (bool): the attention-dropout mask the kernels apply for (dropout_p, seed).
@@ -631,36 +664,58 @@ void check_fp8_source(const at::Tensor& x, const char* name) {
   TORCH_CHECK(x.numel() == 0 || x.size(1) == 1 || x.stride(1) == 1, "fp8: rows of ", name, " must be contiguous");
   TORCH_CHECK(x.numel() == 0 || x.size(0) == 1 || x.stride(0) >= x.size(1), "fp8: rows of ", name, " must not overlap");
   TORCH_CHECK(x.size(0) <= (1 << 22) && x.size(1) <= (1 << 22), "fp8: ", name, " is larger than 2^22 rows or columns");
+  TORCH_CHECK(((x.size(0) + 127) / 128) * ((x.size(1) + 127) / 128) < (1 << 29), "fp8: ", name, " has too many tiles");
 }
 
-// Quantises x [R, C] by rows and / or columns, or by tiles (then both layouts share the scales). An output
-// that is not wanted stays undefined. `sums`: fp32 [ceil(R / 128), C] partial column sums (not with tiles).
-void fp8_quantize_into(const at::Tensor& x, bool tiles, Fp8Pair* rows, Fp8Pair* cols, at::Tensor* sums) {
-  const int64_t R = x.size(0), C = x.size(1), Rb = (R + 127) / 128, Cb = (C + 127) / 128;
-  const auto q8 = x.options().dtype(at::kFloat8_e4m3fn), u8 = x.options().dtype(at::kByte);
-  if (rows) {
-    rows->q = at::empty({R, Cb * 128}, q8);
-    rows->scale = at::empty({tiles ? Rb : R, round_up(Cb, 4)}, u8);
-  }
-  if (cols) {
-    cols->q = at::empty({C, Rb * 128}, q8);
-    cols->scale = at::empty({tiles ? Cb : C, round_up(Rb, 4)}, u8);
-  }
-  if (sums) *sums = at::empty({Rb, C}, x.options().dtype(at::kFloat));
-  if (R == 0 || C == 0) return;  // every output is empty
-  auto bytes = [](const at::Tensor& t) { return reinterpret_cast<uint8_t*>(t.data_ptr()); };
-  pda::fp8_quantize(dtype_of(x), x.data_ptr(), R > 1 ? x.stride(0) : C, (int)R, (int)C, tiles, rows ? bytes(rows->q) : nullptr,
-                    rows ? bytes(rows->scale) : nullptr, cols ? bytes(cols->q) : nullptr,
-                    cols ? bytes(cols->scale) : nullptr, sums ? sums->data_ptr<float>() : nullptr, current_stream());
-  check_launch("fp8_quantize");
+// `x` [..., C] as a matrix [rows, C] that check_fp8_source accepts, copied only if it has to be.
+at::Tensor fp8_source(const at::Tensor& x) {
+  at::Tensor m = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
+  const bool ok = (m.size(1) <= 1 || m.stride(1) == 1) && (m.size(0) <= 1 || m.stride(0) >= m.size(1));
+  return ok ? m : m.contiguous();
 }
+
+// Matrices to be quantised in one launch.
+struct Fp8Quantizer {
+  pda::Fp8QuantProblem problems[3];
+  int n = 0;
+  pda::DType dtype = pda::kBF16;
+
+  // x [R, C] by rows and / or columns, or by tiles (then both layouts share the scales); an output that is not
+  // wanted is null. `sums`: fp32 [ceil(R / 128), C] partial column sums (not with tiles).
+  void add(const at::Tensor& x, bool tiles, Fp8Pair* rows, Fp8Pair* cols, at::Tensor* sums) {
+    const int64_t R = x.size(0), C = x.size(1), Rb = (R + 127) / 128, Cb = (C + 127) / 128;
+    const auto q8 = x.options().dtype(at::kFloat8_e4m3fn), u8 = x.options().dtype(at::kByte);
+    if (rows) {
+      rows->q = at::empty({R, Cb * 128}, q8);
+      rows->scale = at::empty({tiles ? Rb : R, round_up(Cb, 4)}, u8);
+    }
+    if (cols) {
+      cols->q = at::empty({C, Rb * 128}, q8);
+      cols->scale = at::empty({tiles ? Cb : C, round_up(Rb, 4)}, u8);
+    }
+    if (sums) *sums = at::empty({Rb, C}, x.options().dtype(at::kFloat));
+    if (R == 0 || C == 0) return;  // every output is empty
+    auto bytes = [](const at::Tensor& t) { return reinterpret_cast<uint8_t*>(t.data_ptr()); };
+    dtype = dtype_of(x);
+    problems[n++] = {x.data_ptr(), R > 1 ? x.stride(0) : C, (int)R, (int)C, tiles, rows ? bytes(rows->q) : nullptr,
+                     rows ? bytes(rows->scale) : nullptr, cols ? bytes(cols->q) : nullptr,
+                     cols ? bytes(cols->scale) : nullptr, sums ? sums->data_ptr<float>() : nullptr};
+  }
+  void run() {
+    if (n == 0) return;
+    pda::fp8_quantize(dtype, problems, n, current_stream());
+    check_launch("fp8_quantize");
+  }
+};
 
 std::vector<at::Tensor> fp8_quantize(const at::Tensor& x, bool want_rows, bool want_cols, bool tiles) {
   check_fp8_source(x, "x");
   TORCH_CHECK(want_rows || want_cols, "fp8_quantize: no output asked for");
   const c10::DeviceGuard guard(x.device());
   Fp8Pair rows, cols;
-  fp8_quantize_into(x, tiles, want_rows ? &rows : nullptr, want_cols ? &cols : nullptr, nullptr);
+  Fp8Quantizer quantizer;
+  quantizer.add(x, tiles, want_rows ? &rows : nullptr, want_cols ? &cols : nullptr, nullptr);
+  quantizer.run();
   std::vector<at::Tensor> out;
   if (want_rows) out.insert(out.end(), {rows.q, rows.scale});
   if (want_cols) out.insert(out.end(), {cols.q, cols.scale});
@@ -684,101 +739,133 @@ pda::Fp8Operand fp8_operand(const at::Tensor& q, const at::Tensor& scale, bool t
   return pda::Fp8Operand{q.data_ptr(), scale.data_ptr(), Kp, scale.size(1), (int)rows, tiles};
 }
 
-// out[M, N] = (out +) bias + x . w^T; `out` fresh in `dtype` unless given.
-at::Tensor fp8_product(const Fp8Pair& x, bool x_tiles, const Fp8Pair& w, bool w_tiles, int64_t K,
-                       const std::optional<at::Tensor>& bias, at::ScalarType dtype, const std::optional<at::Tensor>& out,
-                       bool accumulate) {
-  const pda::Fp8Operand X = fp8_operand(x.q, x.scale, x_tiles, K, "the left operand");
-  const pda::Fp8Operand W = fp8_operand(w.q, w.scale, w_tiles, K, "the right operand");
-  TORCH_CHECK(x.q.device() == w.q.device(), "fp8_matmul: operands on different devices");
-  const int64_t M = X.rows, N = W.rows;
-  at::Tensor y;
-  if (out.has_value()) {
-    y = *out;
-    TORCH_CHECK(y.device() == x.q.device() && y.is_contiguous() && y.numel() == M * N, "fp8_matmul: out must be a contiguous tensor with ",
-                M * N, " elements on the operands' device");
-  } else {
-    TORCH_CHECK(!accumulate, "fp8_matmul: accumulate needs an out tensor");
-    TORCH_CHECK(dtype == at::kBFloat16 || dtype == at::kFloat, "fp8_matmul: out dtype must be bfloat16 or float32, got ", dtype);
-    y = at::empty({M, N}, x.q.options().dtype(dtype));
-  }
-  const pda::DType out_dtype = dtype_of(y);
-  if (bias.has_value())
-    TORCH_CHECK(bias->device() == x.q.device() && bias->is_contiguous() && bias->numel() == N, "fp8_matmul: bias must be a contiguous tensor with ",
-                N, " elements on the operands' device");
-  const pda::DType bias_dtype = bias.has_value() ? dtype_of(*bias) : pda::kBF16;
-  if (M == 0 || N == 0) return y;
-  if (K == 0) {  // a sum over nothing
-    if (!accumulate) y.zero_();
-    if (bias.has_value()) y.view({M, N}).add_(*bias);
+// Independent products in one launch, their partial sums (and column sums) folded in another.
+struct Fp8Products {
+  pda::Fp8GemmProblem problems[2];
+  int n = 0;
+  std::vector<at::Tensor> partials;
+
+  // out[M, N] = (out +) bias + x . w^T over K; `out` fresh in `dtype` unless given.
+  at::Tensor add(const Fp8Pair& x, bool x_tiles, const Fp8Pair& w, bool w_tiles, int64_t K, const std::optional<at::Tensor>& bias,
+                 at::ScalarType dtype, const std::optional<at::Tensor>& out, bool accumulate) {
+    const pda::Fp8Operand X = fp8_operand(x.q, x.scale, x_tiles, K, "the left operand");
+    const pda::Fp8Operand W = fp8_operand(w.q, w.scale, w_tiles, K, "the right operand");
+    TORCH_CHECK(x.q.device() == w.q.device(), "fp8_matmul: operands on different devices");
+    const int64_t M = X.rows, N = W.rows;
+    at::Tensor y;
+    if (out.has_value()) {
+      y = *out;
+      TORCH_CHECK(y.device() == x.q.device() && y.is_contiguous() && y.numel() == M * N, "fp8_matmul: out must be a contiguous tensor with ",
+                  M * N, " elements on the operands' device");
+    } else {
+      TORCH_CHECK(!accumulate, "fp8_matmul: accumulate needs an out tensor");
+      TORCH_CHECK(dtype == at::kBFloat16 || dtype == at::kFloat, "fp8_matmul: out dtype must be bfloat16 or float32, got ", dtype);
+      y = at::empty({M, N}, x.q.options().dtype(dtype));
+    }
+    const pda::DType out_dtype = dtype_of(y);
+    if (bias.has_value())
+      TORCH_CHECK(bias->device() == x.q.device() && bias->is_contiguous() && bias->numel() == N, "fp8_matmul: bias must be a contiguous tensor with ",
+                  N, " elements on the operands' device");
+    const pda::DType bias_dtype = bias.has_value() ? dtype_of(*bias) : pda::kBF16;
+    if (M == 0 || N == 0) return y;
+    if (K == 0) {  // a sum over nothing
+      if (!accumulate) y.zero_();
+      if (bias.has_value()) y.view({M, N}).add_(*bias);
+      return y;
+    }
+    const pda::Fp8GemmPlan plan = pda::fp8_gemm_plan((int)M, (int)N, (int)X.ld, out_dtype);
+    float* partial = nullptr;
+    if (plan.slices > 1 || accumulate) {
+      partials.push_back(at::empty({plan.slices, M, N}, x.q.options().dtype(at::kFloat)));
+      partial = partials.back().data_ptr<float>();
+    }
+    problems[n++] = {X, W, (int)X.ld, bias.has_value() ? bias->data_ptr() : nullptr, bias_dtype, y.data_ptr(), out_dtype, accumulate, plan, partial};
     return y;
   }
-  const pda::Fp8GemmPlan plan = pda::fp8_gemm_plan((int)M, (int)N, (int)X.ld, out_dtype);
-  at::Tensor partial;
-  if (plan.slices > 1) partial = at::empty({plan.slices, M, N}, x.q.options().dtype(at::kFloat));
-  pda::fp8_gemm(X, W, (int)X.ld, bias.has_value() ? bias->data_ptr() : nullptr, bias_dtype, y.data_ptr(), out_dtype, accumulate,
-                plan, plan.slices > 1 ? partial.data_ptr<float>() : nullptr, current_stream());
-  check_launch("fp8_gemm");
-  return y;
-}
+  void run(const pda::Fp8ColumnSums* sums = nullptr) {
+    if (n == 0 && !sums) return;
+    pda::fp8_gemm(problems, n, sums, current_stream());
+    check_launch("fp8_gemm");
+  }
+};
 
 at::Tensor fp8_matmul(const at::Tensor& xq, const at::Tensor& xs, bool x_tiles, const at::Tensor& wq, const at::Tensor& ws,
                       bool w_tiles, int64_t K, const std::optional<at::Tensor>& bias, bool out_f32) {
   TORCH_CHECK(xq.is_cuda(), "fp8_matmul: operands must live on the GPU");
   const c10::DeviceGuard guard(xq.device());
-  return fp8_product({xq, xs}, x_tiles, {wq, ws}, w_tiles, K, bias, out_f32 ? at::kFloat : at::kBFloat16, std::nullopt, false);
+  Fp8Products products;
+  at::Tensor y = products.add({xq, xs}, x_tiles, {wq, ws}, w_tiles, K, bias, out_f32 ? at::kFloat : at::kBFloat16, std::nullopt, false);
+  products.run();
+  return y;
 }
 
-// y = x . w^T + bias with x [M, K] quantised by rows and w [N, K] by tiles. `keep`: also x quantised by
+// y = x . w^T + bias with x [..., K] quantised by rows and w [N, K] by tiles. `keep`: also x quantised by
 // columns (from the same read of x), which is all that the weight gradient needs of it.
 std::vector<at::Tensor> fp8_linear_forward(const at::Tensor& x, const at::Tensor& weight, const std::optional<at::Tensor>& bias,
                                            bool keep) {
-  check_fp8_source(x, "x");
-  check_fp8_source(weight, "weight");
-  TORCH_CHECK(x.scalar_type() == weight.scalar_type() && x.device() == weight.device() && x.size(1) == weight.size(1),
-              "fp8_linear: x ", x.sizes(), " ", x.scalar_type(), " and weight ", weight.sizes(), " ", weight.scalar_type(), " do not match");
+  const at::Tensor x2 = fp8_source(x), w2 = fp8_source(weight);
+  check_fp8_source(x2, "x");
+  check_fp8_source(w2, "weight");
+  TORCH_CHECK(x2.scalar_type() == w2.scalar_type() && x2.device() == w2.device() && x2.size(1) == w2.size(1), "fp8_linear: x ",
+              x.sizes(), " ", x.scalar_type(), " and weight ", weight.sizes(), " ", weight.scalar_type(), " do not match");
   const c10::DeviceGuard guard(x.device());
   Fp8Pair xr, xc, wr;
-  fp8_quantize_into(x, false, &xr, keep ? &xc : nullptr, nullptr);
-  fp8_quantize_into(weight, true, &wr, nullptr, nullptr);
-  at::Tensor y = fp8_product(xr, false, wr, true, x.size(1), bias, x.scalar_type(), std::nullopt, false);
+  Fp8Quantizer quantizer;
+  quantizer.add(x2, false, &xr, keep ? &xc : nullptr, nullptr);
+  quantizer.add(w2, true, &wr, nullptr, nullptr);
+  quantizer.run();
+  Fp8Products products;
+  std::optional<at::Tensor> b;
+  if (bias.has_value()) b = bias->contiguous();
+  at::Tensor y = products.add(xr, false, wr, true, x2.size(1), b, x.scalar_type(), std::nullopt, false);
+  products.run();
+  std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+  shape.back() = weight.size(0);
+  y = y.view(shape);
   if (keep) return {y, xc.q, xc.scale};
   return {y};
 }
 
 // Gradients of that: dx = dy . w (dy by rows, w by tiles), dw = dy^T . x (both by columns), db = column sums of
 // dy before quantisation. xq / xs: x by columns (fp8_linear_forward's `keep`), or `x` itself, quantised here.
+// dx has dy's leading dimensions.
 std::vector<at::Tensor> fp8_linear_backward(const at::Tensor& dy, const at::Tensor& weight, const std::optional<at::Tensor>& x,
                                             const std::optional<at::Tensor>& xq, const std::optional<at::Tensor>& xs, bool want_x,
                                             bool want_w, bool want_b, const std::optional<at::Tensor>& w_out, bool w_accumulate,
                                             const std::optional<at::Tensor>& b_out, bool b_accumulate) {
-  check_fp8_source(dy, "dy");
-  check_fp8_source(weight, "weight");
-  const int64_t M = dy.size(0), N = dy.size(1), K = weight.size(1);
-  TORCH_CHECK(dy.scalar_type() == weight.scalar_type() && dy.device() == weight.device() && weight.size(0) == N,
+  const at::Tensor g2 = fp8_source(dy), w2 = fp8_source(weight);
+  check_fp8_source(g2, "dy");
+  check_fp8_source(w2, "weight");
+  const int64_t M = g2.size(0), N = g2.size(1), K = w2.size(1);
+  TORCH_CHECK(dy.scalar_type() == weight.scalar_type() && dy.device() == weight.device() && w2.size(0) == N,
               "fp8_linear backward: dy ", dy.sizes(), " ", dy.scalar_type(), " and weight ", weight.sizes(), " ", weight.scalar_type(), " do not match");
   const c10::DeviceGuard guard(dy.device());
   Fp8Pair gr, gc, wc, xc;
-  at::Tensor sums, dx, dw, db;
+  at::Tensor sums, dx, dw, db, x2;
+  Fp8Quantizer quantizer;
   if (want_x || want_w || want_b)  // (the bias gradient alone still needs the pass: rows are the cheaper by-product)
-    fp8_quantize_into(dy, false, want_x || !want_w ? &gr : nullptr, want_w ? &gc : nullptr, want_b ? &sums : nullptr);
+    quantizer.add(g2, false, want_x || !want_w ? &gr : nullptr, want_w ? &gc : nullptr, want_b ? &sums : nullptr);
+  if (want_x) quantizer.add(w2, true, nullptr, &wc, nullptr);
+  if (want_w && x.has_value()) {
+    x2 = fp8_source(*x);
+    check_fp8_source(x2, "x");
+    TORCH_CHECK(x2.size(0) == M && x2.size(1) == K && x2.scalar_type() == dy.scalar_type() && x2.device() == dy.device(),
+                "fp8_linear backward: x ", x->sizes(), " does not match dy ", dy.sizes());
+    quantizer.add(x2, false, nullptr, &xc, nullptr);
+  } else if (want_w) {
+    TORCH_CHECK(xq.has_value() && xs.has_value(), "fp8_linear backward: the weight gradient needs x");
+    xc = {*xq, *xs};
+  }
+  quantizer.run();
+  Fp8Products products;
   if (want_x) {
-    fp8_quantize_into(weight, true, nullptr, &wc, nullptr);
-    dx = fp8_product(gr, false, wc, true, N, std::nullopt, dy.scalar_type(), std::nullopt, false);
+    dx = products.add(gr, false, wc, true, N, std::nullopt, dy.scalar_type(), std::nullopt, false);
+    std::vector<int64_t> shape(dy.sizes().begin(), dy.sizes().end());
+    shape.back() = K;
+    dx = dx.view(shape);
   }
-  if (want_w) {
-    if (x.has_value()) {
-      check_fp8_source(*x, "x");
-      TORCH_CHECK(x->size(0) == M && x->size(1) == K && x->scalar_type() == dy.scalar_type() && x->device() == dy.device(),
-                  "fp8_linear backward: x ", x->sizes(), " does not match dy ", dy.sizes());
-      fp8_quantize_into(*x, false, nullptr, &xc, nullptr);
-    } else {
-      TORCH_CHECK(xq.has_value() && xs.has_value(), "fp8_linear backward: the weight gradient needs x");
-      xc = {*xq, *xs};
-    }
-    dw = fp8_product(gc, false, xc, false, M, std::nullopt, dy.scalar_type(), w_out, w_accumulate);
-    if (!w_out.has_value()) dw = dw.view({N, K});
-  }
+  if (want_w) dw = products.add(gc, false, xc, false, M, std::nullopt, dy.scalar_type(), w_out, w_accumulate);
+  pda::Fp8ColumnSums fold{};
   if (want_b) {
     if (b_out.has_value()) {
       db = *b_out;
@@ -788,13 +875,37 @@ std::vector<at::Tensor> fp8_linear_backward(const at::Tensor& dy, const at::Tens
       TORCH_CHECK(!b_accumulate, "fp8_linear backward: accumulating the bias gradient needs its tensor");
       db = at::empty({N}, dy.options());
     }
-    if (N > 0) {
-      pda::fp8_fold_column_sums(M > 0 ? sums.data_ptr<float>() : nullptr, (int)((M + 127) / 128), (int)N, dtype_of(db), db.data_ptr(),
-                                b_accumulate, current_stream());
-      check_launch("fp8_fold_column_sums");
-    }
+    fold = {M > 0 ? sums.data_ptr<float>() : nullptr, (int)((M + 127) / 128), (int)N, db.data_ptr(), dtype_of(db), b_accumulate};
   }
+  products.run(want_b && N > 0 ? &fold : nullptr);
   return {dx, dw, db};
+}
+
+// The layer as one autograd node, for gradients that autograd itself takes (no gradient sink, no recipe for x).
+struct Fp8LinearFn : public torch::autograd::Function<Fp8LinearFn> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight,
+                            const std::optional<at::Tensor>& bias, bool keep) {
+    std::vector<at::Tensor> got = fp8_linear_forward(x, weight, bias, keep);
+    if (keep) ctx->save_for_backward({weight, got[1], got[2]});
+    else ctx->save_for_backward({weight});
+    ctx->saved_data["bias"] = bias.has_value();
+    return got[0];
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "fp8_linear has no second derivative (create_graph=True)");
+    const auto saved = ctx->get_saved_variables();
+    const bool keep = saved.size() == 3;
+    const bool want_b = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(2);
+    std::optional<at::Tensor> xq, xs;
+    if (keep) xq = saved[1], xs = saved[2];
+    auto got = fp8_linear_backward(grads[0], saved[0], std::nullopt, xq, xs, ctx->needs_input_grad(0), keep && ctx->needs_input_grad(1),
+                                   want_b, std::nullopt, false, std::nullopt, false);
+    return {got[0], got[1], got[2], at::Tensor()};
+  }
+};
+
+at::Tensor fp8_linear(const at::Tensor& x, const at::Tensor& weight, const std::optional<at::Tensor>& bias) {
+  return Fp8LinearFn::apply(x, weight, bias, at::GradMode::is_enabled() && weight.requires_grad());
 }
 
 }  // namespace
@@ -970,6 +1081,7 @@ void bind_ops(py::module_& m) {
   m.def("fp8_quantize", &fp8_quantize, py::arg("x"), py::arg("rows"), py::arg("columns"), py::arg("tiles"));
   m.def("fp8_matmul", &fp8_matmul, py::arg("xq"), py::arg("xs"), py::arg("x_tiles"), py::arg("wq"), py::arg("ws"),
         py::arg("w_tiles"), py::arg("K"), py::arg("bias"), py::arg("out_f32"));
+  m.def("fp8_linear", &fp8_linear, py::arg("x"), py::arg("weight"), py::arg("bias"));
   m.def("fp8_linear_forward", &fp8_linear_forward, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("keep"));
   m.def("fp8_linear_backward", &fp8_linear_backward, py::arg("dy"), py::arg("weight"), py::arg("x"), py::arg("xq"), py::arg("xs"),
         py::arg("want_x"), py::arg("want_w"), py::arg("want_b"), py::arg("w_out"), py::arg("w_accumulate"), py::arg("b_out"),
@@ -979,6 +1091,8 @@ void bind_ops(py::module_& m) {
   m.def("attention_backward", &attention_backward, py::arg("qkv"), py::arg("out"), py::arg("dout"),
         py::arg("lse"), py::arg("num_heads"), py::arg("softmax_scale"), py::arg("dropout_p") = 0.0,
         py::arg("seed") = 0);
+  m.def("window_attention", &window_attention, py::arg("qkv"), py::arg("num_heads"), py::arg("window"), py::arg("sinks"),
+        py::arg("softmax_scale"), py::arg("dropout_p"), py::arg("seed"));
   m.def("window_attention_forward", &window_attention_forward, py::arg("qkv"), py::arg("num_heads"), py::arg("window"),
         py::arg("sinks"), py::arg("softmax_scale"), py::arg("dropout_p"), py::arg("seed"));
   m.def("window_attention_backward", &window_attention_backward, py::arg("qkv"), py::arg("out"), py::arg("dout"), py::arg("lse"),

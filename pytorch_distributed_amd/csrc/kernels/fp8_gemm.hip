@@ -29,6 +29,8 @@
 //
 // Few output tiles (weight gradients, few tokens): the contraction is cut into slices of whole 512-value
 // scale groups, fp32 partial tiles are folded in slice order by a second kernel (deterministic).
+#include <type_traits>
+
 #include "attention_common.h"
 #include "pda_kernels.h"
 
@@ -96,16 +98,22 @@ struct Operand {
   int rows, shift;
 };
 
-struct Output {
-  void* ptr;         // [M, N] (bf16 or fp32), or the fp32 partials [slices][M][N]
+struct Problem {
+  Operand x, w;
+  void* out;         // [M, N] (bf16 or fp32), or the fp32 partials [slices][M][N]
   const void* bias;  // [N] or null
-  int64_t ld;
-  bool bias_f32, accumulate, vec;  // vec: rows are aligned for four-value stores
+  bool out_f32, bias_f32, vec;  // vec: rows are 16-byte aligned
+  int steps, steps_per_slice, tasks;
 };
 
-template <int kWB, typename Out, bool kWide>
-__global__ __launch_bounds__(kThreads) void fp8_gemm_kernel(Operand X, Operand W, Output O, int steps_total,
-                                                            int steps_per_slice) {
+// Up to two independent products in one launch (the two gradients of a layer): problem 1's workgroups follow
+// problem 0's, padded to a multiple of 8 so that both see their XCD as blockIdx % 8.
+struct Problems {
+  Problem p[2];
+};
+
+template <int kWB, bool kWide>
+__global__ __launch_bounds__(kThreads) void fp8_gemm_kernel(const Problems P) {
   constexpr int kTile = 64 * kWB;
   constexpr int kSlab = kTile * kStageK;       // bytes of one operand's stage
   constexpr int kStageBytes = 2 * kSlab;
@@ -114,20 +122,27 @@ __global__ __launch_bounds__(kThreads) void fp8_gemm_kernel(Operand X, Operand W
   constexpr int kScaleBytes = 2 * kTile * 4;   // one group's scales: X rows, then W rows
   extern __shared__ __attribute__((aligned(16))) char smem[];
   char* scale_smem = smem + kStages * kStageBytes;
+  float* bias_smem = reinterpret_cast<float*>(scale_smem + 2 * kScaleBytes);
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = wave >> 1, wj = wave & 1;
   const int r = lane & 31, h = lane >> 5;
+
+  const int padded0 = (P.p[0].tasks + 7) & ~7;
+  const bool second = (int)blockIdx.x >= padded0;
+  const Problem& pr = P.p[second];
+  const int local = blockIdx.x - (second ? padded0 : 0);
+  if (local >= pr.tasks) return;  // padding
+  const Operand &X = pr.x, &W = pr.w;
   const int M = X.rows, N = W.rows;
 
   // Tasks are dealt to the 8 XCDs in contiguous ranges; consecutive tasks walk kGroupM token tiles x all
   // feature tiles, so the workgroups of an XCD share operand rows in its L2.
   const int tiles_m = (M + kTile - 1) / kTile, tiles_n = (N + kTile - 1) / kTile;
   const int n_tiles = tiles_m * tiles_n;
-  const int n_tasks = gridDim.x;
-  const int q8 = n_tasks / 8, r8 = n_tasks % 8;
-  const int xcd = blockIdx.x % 8, within = blockIdx.x / 8;
+  const int q8 = pr.tasks / 8, r8 = pr.tasks % 8;
+  const int xcd = local % 8, within = local / 8;
   const int task = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + within;
   const int slice = task / n_tiles;
   const int tile = task - slice * n_tiles;
@@ -136,8 +151,15 @@ __global__ __launch_bounds__(kThreads) void fp8_gemm_kernel(Operand X, Operand W
   const int group_rows = min(kGroupM, tiles_m - group * kGroupM);
   const int m0 = (group * kGroupM + in_group % group_rows) * kTile;
   const int n0 = (in_group / group_rows) * kTile;
-  const int first = slice * steps_per_slice;  // a multiple of kGroupStages
-  const int n_steps = min(steps_per_slice, steps_total - first);
+  const int first = slice * pr.steps_per_slice;  // a multiple of kGroupStages
+  const int n_steps = min(pr.steps_per_slice, pr.steps - first);
+
+  for (int i = threadIdx.x; i < kTile; i += kThreads) {  // read by the epilogue, many barriers from here
+    float v = 0.f;
+    if (pr.bias && n0 + i < N)
+      v = pr.bias_f32 ? ((const float*)pr.bias)[n0 + i] : bf16_to_f32(((const bf16_raw*)pr.bias)[n0 + i]);
+    bias_smem[i] = v;
+  }
 
   // ---- staging: piece i of a slab = rows (kTile / 4) wave + 16 i .. +15, lane p -> row + p / 4, slot p % 4.
   // Rows past the end repeat the last one (never stored).
@@ -301,75 +323,153 @@ __global__ __launch_bounds__(kThreads) void fp8_gemm_kernel(Operand X, Operand W
     take_scales();
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the tail's unused loads have left LDS alone
+  __syncthreads();                                  // and nobody reads the ring any more: it stages the output
 
   // ---- epilogue: register e of acc[a][b]: token m0 + 32 kWB wi + 32 a + r, feature n0 + 32 kWB wj + 32 b +
-  // 8 (e / 4) + 4 h + (e & 3)
-  Out* out = (Out*)O.ptr + int64_t(slice) * M * N;
+  // 8 (e / 4) + 4 h + (e & 3). Through LDS, so that rows leave in whole lines: staged row = token, its 16-byte
+  // chunks XOR-permuted with the token, so the lanes of a write (32 tokens, one feature offset) and of a read
+  // (one token) both spread over the banks. Written in `passes` passes of the a-blocks that fit the ring.
+  auto store_tile = [&](auto out_f32, auto passes) {
+    using Out = std::conditional_t<decltype(out_f32)::value, float, bf16_raw>;
+    constexpr int kRowBytes = kTile * (int)sizeof(Out), kVec = 16 / (int)sizeof(Out);
+    constexpr int kPasses = decltype(passes)::value, kBlocks = kWB / kPasses, kRows = 64 * kBlocks;
+    constexpr int kChunks = kRowBytes / 16;
+    Out* out = (Out*)pr.out + int64_t(slice) * M * N;
 #pragma unroll
-  for (int b = 0; b < kWB; ++b)
+    for (int pass = 0; pass < kPasses; ++pass) {
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const int n = n0 + 32 * (kWB * wj + b) + 8 * g + 4 * h;
-      float bv[4] = {0.f, 0.f, 0.f, 0.f};
-      if (O.bias) {
+      for (int ai = 0; ai < kBlocks; ++ai)
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (n + e < N) bv[e] = O.bias_f32 ? ((const float*)O.bias)[n + e] : bf16_to_f32(((const bf16_raw*)O.bias)[n + e]);
-      }
+        for (int b = 0; b < kWB; ++b) {
+          f32x16 v = acc[pass * kBlocks + ai][b];
+          asm volatile("" : "+v"(v));  // one block at a time leaves the accumulator file
+          const int row = 32 * (kBlocks * wi + ai) + r;
 #pragma unroll
-      for (int a = 0; a < kWB; ++a) {
-        const int m = m0 + 32 * (kWB * wi + a) + r;
-        if (m >= M) continue;
-        Out* dst = out + int64_t(m) * O.ld + n;
-        float v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = acc[a][b][4 * g + e] + bv[e];
-        if (O.accumulate) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (n + e < N) v[e] += VecIO<Out>::load1(dst + e);
-        }
-        if (O.vec && n + 4 <= N) {
-          if constexpr (sizeof(Out) == 2) {
-            *reinterpret_cast<u32x2*>(dst) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-          } else {
-            *reinterpret_cast<f32x4*>(dst) = f32x4{v[0], v[1], v[2], v[3]};
+          for (int g = 0; g < 4; ++g) {
+            const int col = 32 * (kWB * wj + b) + 8 * g + 4 * h;
+            const f32x4 bv = *reinterpret_cast<const f32x4*>(bias_smem + col);
+            const int at = row * kRowBytes + (((col / kVec) ^ (r & (kChunks - 1))) * 16) + (col % kVec) * (int)sizeof(Out);
+            if constexpr (sizeof(Out) == 2)
+              *reinterpret_cast<u32x2*>(smem + at) = u32x2{pack_bf16x2(v[4 * g] + bv[0], v[4 * g + 1] + bv[1]),
+                                                          pack_bf16x2(v[4 * g + 2] + bv[2], v[4 * g + 3] + bv[3])};
+            else
+              *reinterpret_cast<f32x4*>(smem + at) = f32x4{v[4 * g] + bv[0], v[4 * g + 1] + bv[1], v[4 * g + 2] + bv[2], v[4 * g + 3] + bv[3]};
           }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (n + e < N) VecIO<Out>::store1(dst + e, v[e]);
+        }
+      __syncthreads();
+      // staged row q is token 32 kWB (q / 32 / kBlocks) + 32 (pass kBlocks + q / 32 % kBlocks) + q % 32 of the tile
+      auto token = [&](int q) {
+        const int blk = q >> 5;
+        return m0 + 32 * (kWB * (blk / kBlocks) + pass * kBlocks + blk % kBlocks) + (q & 31);
+      };
+      if (pr.vec) {
+        const int ch = threadIdx.x % kChunks, n = n0 + ch * kVec;
+        if (n < N) {  // (rows are whole chunks here)
+#pragma unroll 4
+          for (int q = threadIdx.x / kChunks; q < kRows; q += kThreads / kChunks) {
+            const int m = token(q);
+            const u32x4 w = *reinterpret_cast<const u32x4*>(smem + q * kRowBytes + ((ch ^ (q & 31 & (kChunks - 1))) * 16));
+            if (m < M) *reinterpret_cast<u32x4*>(out + int64_t(m) * N + n) = w;
+          }
+        }
+      } else {  // rows at any alignment: an element per lane, neighbours in neighbouring lanes
+        const int col = threadIdx.x % kTile, n = n0 + col;
+        if (n < N) {
+#pragma unroll 4
+          for (int q = threadIdx.x / kTile; q < kRows; q += kThreads / kTile) {
+            const int m = token(q);
+            const Out w = *reinterpret_cast<const Out*>(smem + q * kRowBytes + (((col / kVec) ^ (q & 31 & (kChunks - 1))) * 16) +
+                                                        (col % kVec) * (int)sizeof(Out));
+            if (m < M) out[int64_t(m) * N + n] = w;
+          }
         }
       }
+      if (pass + 1 < kPasses) __syncthreads();
     }
-}
-
-// out = (out +) bias + sum over slices, in slice order.
-template <typename Out>
-__global__ __launch_bounds__(kThreads) void fold_slices_kernel(const float* __restrict__ partial, int slices, int64_t total,
-                                                               int N, const void* __restrict__ bias, bool bias_f32,
-                                                               Out* __restrict__ out, bool accumulate) {
-  const int64_t i = int64_t(blockIdx.x) * kThreads + threadIdx.x;
-  if (i >= total) return;
-  float v = 0.f;
-  for (int s = 0; s < slices; ++s) v += partial[s * total + i];
-  if (bias) {
-    const int n = int(i % N);
-    v += bias_f32 ? ((const float*)bias)[n] : bf16_to_f32(((const bf16_raw*)bias)[n]);
+  };
+  if constexpr (kWide) {
+    store_tile(std::true_type{}, std::integral_constant<int, 1>{});
+  } else if (pr.out_f32) {
+    store_tile(std::true_type{}, std::integral_constant<int, kWB / 2>{});
+  } else {
+    store_tile(std::false_type{}, std::integral_constant<int, 1>{});
   }
-  if (accumulate) v += VecIO<Out>::load1(out + i);
-  VecIO<Out>::store1(out + i, v);
 }
 
-template <int kWB, typename Out, bool kWide>
-void launch(const Operand& x, const Operand& w, const Output& o, int steps, int steps_per_slice, int slices,
-            hipStream_t stream) {
+// out = (out +) bias + sum over `slices` of partial [slices][total], in a fixed order. Up to three such sums in
+// one launch. `tall`: many slices of few values (column sums): 64 values per workgroup, a quarter of the slices
+// per wave; otherwise four values per thread.
+struct Fold {
+  const float* partial;
+  const void* bias;
+  void* out;
+  int64_t total;
+  int slices, N, blocks;
+  bool bias_f32, out_f32, accumulate, tall;
+};
+struct Folds {
+  Fold f[3];
+};
+
+__global__ __launch_bounds__(kThreads) void fold_kernel(const Folds folds) {
+  __shared__ float red[4][64];
+  int block = blockIdx.x, k = 0;
+  while (block >= folds.f[k].blocks) block -= folds.f[k++].blocks;  // (the blocks' sum is the grid)
+  const Fold& f = folds.f[k];
+  auto finish = [&](int64_t i, float v) {
+    if (f.bias) v += f.bias_f32 ? ((const float*)f.bias)[i % f.N] : bf16_to_f32(((const bf16_raw*)f.bias)[i % f.N]);
+    if (f.out_f32) {
+      float* o = (float*)f.out + i;
+      *o = f.accumulate ? *o + v : v;
+    } else {
+      bf16_raw* o = (bf16_raw*)f.out + i;
+      *o = f32_to_bf16(f.accumulate ? bf16_to_f32(*o) + v : v);
+    }
+  };
+  if (f.tall) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t i = int64_t(block) * 64 + lane;
+    float v = 0.f;
+    if (i < f.total) {
+#pragma unroll 8
+      for (int s = wave; s < f.slices; s += 4) v += f.partial[s * f.total + i];
+    }
+    red[wave][lane] = v;
+    __syncthreads();
+    if (wave == 0 && i < f.total) finish(i, (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]));
+    return;
+  }
+  const int64_t i = (int64_t(block) * kThreads + threadIdx.x) * 4;
+  if (f.total % 4 == 0) {
+    if (i >= f.total) return;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < f.slices; ++s) {
+      const f32x4 p = *reinterpret_cast<const f32x4*>(f.partial + s * f.total + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += p[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) finish(i + e, v[e]);
+    return;
+  }
+  for (int e = 0; e < 4; ++e) {
+    const int64_t at = int64_t(block) * kThreads * 4 + e * kThreads + threadIdx.x;
+    if (at >= f.total) return;
+    float v = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < f.slices; ++s) v += f.partial[s * f.total + at];
+    finish(at, v);
+  }
+}
+
+template <int kWB, bool kWide>
+void launch(const Problems& P, hipStream_t stream) {
   constexpr int kTile = 64 * kWB;
-  constexpr int kLds = kStages * 2 * kTile * kStageK + 2 * 2 * kTile * 4;
-  (void)hipFuncSetAttribute((const void*)fp8_gemm_kernel<kWB, Out, kWide>, hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
-  const int64_t tasks = ceil_div(x.rows, kTile) * ceil_div(w.rows, kTile) * slices;
-  hipLaunchKernelGGL((fp8_gemm_kernel<kWB, Out, kWide>), dim3((unsigned)tasks), dim3(kThreads), kLds, stream, x, w, o, steps,
-                     steps_per_slice);
+  constexpr int kLds = kStages * 2 * kTile * kStageK + 2 * 2 * kTile * 4 + kTile * 4;
+  (void)hipFuncSetAttribute((const void*)fp8_gemm_kernel<kWB, kWide>, hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+  const unsigned blocks = (unsigned)(((P.p[0].tasks + 7) & ~7) + P.p[1].tasks);
+  hipLaunchKernelGGL((fp8_gemm_kernel<kWB, kWide>), dim3(blocks), dim3(kThreads), kLds, stream, P);
 }
 
 }  // namespace
@@ -390,30 +490,50 @@ Fp8GemmPlan fp8_gemm_plan(int M, int N, int K, DType out_dtype) {
   return p;
 }
 
-void fp8_gemm(const Fp8Operand& x, const Fp8Operand& w, int K, const void* bias, DType bias_dtype, void* out,
-              DType out_dtype, bool accumulate, const Fp8GemmPlan& plan, float* partial, hipStream_t stream) {
-  const Operand X{(const uint8_t*)x.q, (const uint8_t*)x.scale, x.ld, x.ld_scale, x.rows, x.tiles ? 7 : 0};
-  const Operand W{(const uint8_t*)w.q, (const uint8_t*)w.scale, w.ld, w.ld_scale, w.rows, w.tiles ? 7 : 0};
-  const int N = w.rows, steps = K / kStageK;
-  const bool split = plan.slices > 1;
-  const DType kind = split ? kF32 : out_dtype;
-  void* dst = split ? (void*)partial : out;
-  const int quad = kind == kBF16 ? 8 : 16;
-  const Output O{dst, split ? nullptr : bias, N, bias_dtype == kF32, !split && accumulate,
-                 N % 4 == 0 && reinterpret_cast<uintptr_t>(dst) % quad == 0};
-  auto go = [&](auto launcher) { launcher(X, W, O, steps, plan.steps_per_slice, plan.slices, stream); };
-  if (out_dtype == kF32) go(launch<2, float, true>);
-  else if (plan.tile == 256) kind == kBF16 ? go(launch<4, bf16_raw, false>) : go(launch<4, float, false>);
-  else kind == kBF16 ? go(launch<2, bf16_raw, false>) : go(launch<2, float, false>);
-  if (!split) return;
-  const int64_t total = int64_t(x.rows) * N;
-  const dim3 grid((unsigned)ceil_div(total, kThreads)), block(kThreads);
-  if (out_dtype == kBF16)
-    hipLaunchKernelGGL(fold_slices_kernel<bf16_raw>, grid, block, 0, stream, partial, plan.slices, total, N, bias,
-                       bias_dtype == kF32, (bf16_raw*)out, accumulate);
-  else
-    hipLaunchKernelGGL(fold_slices_kernel<float>, grid, block, 0, stream, partial, plan.slices, total, N, bias,
-                       bias_dtype == kF32, (float*)out, accumulate);
+void fp8_gemm(const Fp8GemmProblem* problems, int n, const Fp8ColumnSums* sums, hipStream_t stream) {
+  Problem ps[2] = {};
+  Folds folds = {};
+  int n_folds = 0;
+  auto add_fold = [&](Fold f) {
+    f.blocks = (int)(f.tall ? ceil_div(f.total, 64) : ceil_div(f.total, kThreads * 4));
+    folds.f[n_folds++] = f;
+  };
+  for (int i = 0; i < n; ++i) {
+    const Fp8GemmProblem& g = problems[i];
+    auto operand = [](const Fp8Operand& o) {
+      return Operand{(const uint8_t*)o.q, (const uint8_t*)o.scale, o.ld, o.ld_scale, o.rows, o.tiles ? 7 : 0};
+    };
+    const int M = g.x.rows, N = g.w.rows;
+    const bool fold = g.partial != nullptr;
+    const bool f32 = fold || g.out_dtype == kF32;
+    void* out = fold ? (void*)g.partial : g.out;
+    const int64_t tasks = ceil_div(M, g.plan.tile) * ceil_div(N, g.plan.tile) * g.plan.slices;
+    ps[i] = Problem{operand(g.x), operand(g.w), out, fold ? nullptr : g.bias, f32, g.bias_dtype == kF32,
+                    (int64_t(N) * (f32 ? 4 : 2)) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0,
+                    g.K / kStageK, g.plan.steps_per_slice, (int)tasks};
+    if (fold)
+      add_fold(Fold{g.partial, g.bias, g.out, int64_t(M) * N, g.plan.slices, N, 0, g.bias_dtype == kF32, g.out_dtype == kF32,
+                    g.accumulate, false});
+  }
+  auto go = [&](const Problem& a, const Problem* b, int tile, bool wide) {
+    Problems P = {{a, b ? *b : Problem{}}};
+    if (wide) launch<2, true>(P, stream);
+    else if (tile == 256) launch<4, false>(P, stream);
+    else launch<2, false>(P, stream);
+  };
+  auto wide = [&](int i) { return problems[i].out_dtype == kF32; };
+  if (n == 2 && problems[0].plan.tile == problems[1].plan.tile && wide(0) == wide(1)) {
+    go(ps[0], &ps[1], problems[0].plan.tile, wide(0));
+  } else {
+    for (int i = 0; i < n; ++i) go(ps[i], nullptr, problems[i].plan.tile, wide(i));
+  }
+  if (sums)
+    add_fold(Fold{sums->partial, nullptr, sums->out, sums->C, sums->blocks, sums->C, 0, false, sums->out_dtype == kF32,
+                  sums->accumulate, true});
+  if (n_folds == 0) return;
+  unsigned blocks = 0;
+  for (int i = 0; i < n_folds; ++i) blocks += (unsigned)folds.f[i].blocks;
+  hipLaunchKernelGGL(fold_kernel, dim3(blocks), dim3(kThreads), 0, stream, folds);
 }
 
 }  // namespace pda

@@ -14,7 +14,8 @@
 //   tiles     128 x 128, one scale, both layouts                (weights: both contractions)
 // Cp / Rp are C / R rounded up to 128 (padding: zeros), Sc / Sr the block counts rounded up to 4
 // (padding: zero bytes). The column sums of x (a bias gradient) can ride along: fp32 partial sums per
-// 128-row block, folded in block order by fp8_fold_column_sums.
+// 128-row block, folded in a fixed order by fp8_gemm's last launch. Several matrices share a launch: a layer's
+// small ones cost a launch, not their bytes.
 //
 // What bounds it: memory. A workgroup owns a 128 x 128 tile held in registers (8 rows x 8 columns per
 // thread), so x is read once for both layouts; the transposed bytes pass through a swizzled 16 KiB LDS
@@ -52,13 +53,13 @@ __device__ __forceinline__ float finite_abs(float x) {
 }
 
 // Eight values of one row starting at column c (c % 8 == 0); columns >= C and rows >= R read as zeros.
-template <typename T, bool kVec>
-__device__ __forceinline__ void load8(const T* __restrict__ x, int64_t ld, int R, int C, int row, int c, float (&v)[8]) {
+template <typename T>
+__device__ __forceinline__ void load8(const T* __restrict__ x, int64_t ld, bool vec, int R, int C, int row, int c, float (&v)[8]) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = 0.f;
   if (row >= R || c >= C) return;
   const T* p = x + int64_t(row) * ld + c;
-  if (kVec && c + 8 <= C) {
+  if (vec && c + 8 <= C) {
     if constexpr (sizeof(T) == 2) {
       VecIO<T>::load(p, v);
     } else {
@@ -76,26 +77,41 @@ __device__ __forceinline__ void load8(const T* __restrict__ x, int64_t ld, int R
 }
 
 // Thread (g = tid / 16, j = tid % 16) holds rows 8 g .. 8 g + 7 and columns 8 j .. 8 j + 7 of the tile.
-template <typename T, bool kVec, bool kRows, bool kCols, bool kTiles, bool kSums>
-__global__ __launch_bounds__(kThreads) void quantize_kernel(const T* __restrict__ x, int64_t ld, int R, int C,
-                                                            uint8_t* __restrict__ q, uint8_t* __restrict__ s,
-                                                            uint8_t* __restrict__ qt, uint8_t* __restrict__ st,
-                                                            float* __restrict__ sums) {
-  __shared__ __attribute__((aligned(16))) uint8_t tile[kCols ? kBlock * kBlock : 16];
+struct Matrix {
+  const void* x;
+  int64_t ld;
+  int R, C, blocks;
+  bool vec, tiles;  // vec: rows are 16-byte aligned
+  uint8_t *q, *s, *qt, *st;  // null: not wanted
+  float* sums;
+};
+struct Matrices {
+  Matrix m[3];
+};
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void quantize_kernel(const Matrices all) {
+  __shared__ __attribute__((aligned(16))) uint8_t tile[kBlock * kBlock];
   __shared__ float red[4][kBlock];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int g = tid >> 4, j = tid & 15;
-  const int cb = blockIdx.x, rb = blockIdx.y;
+  int block = blockIdx.x, which = 0;
+  while (block >= all.m[which].blocks) block -= all.m[which++].blocks;  // (the blocks' sum is the grid)
+  const Matrix& mat = all.m[which];
+  const T* __restrict__ x = (const T*)mat.x;
+  const int R = mat.R, C = mat.C;
   const int n_cb = (C + kBlock - 1) / kBlock, n_rb = (R + kBlock - 1) / kBlock;
+  const int rb = block / n_cb, cb = block - rb * n_cb;
   const int row0 = rb * kBlock + 8 * g, col0 = cb * kBlock + 8 * j;
+  uint8_t *const q = mat.q, *const s = mat.s, *const qt = mat.qt, *const st = mat.st;
 
   float v[8][8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) load8<T, kVec>(x, ld, R, C, row0 + i, col0, v[i]);
+  for (int i = 0; i < 8; ++i) load8<T>(x, mat.ld, mat.vec, R, C, row0 + i, col0, v[i]);
 
   float tile_inv = 1.f;
   uint32_t tile_byte = 0;
-  if constexpr (kTiles) {
+  if (mat.tiles) {
     float m = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -106,13 +122,13 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const T* __restrict_
     tile_inv = inverse_scale(tile_byte);
     // one byte per tile in each orientation; the last tile of a row of tiles also clears the padding
     if (tid == 0) {
-      if (kRows) {
+      if (q) {
         const int pitch = (n_cb + 3) & ~3;
         s[int64_t(rb) * pitch + cb] = uint8_t(tile_byte);
         if (cb == n_cb - 1)
           for (int k = n_cb; k < pitch; ++k) s[int64_t(rb) * pitch + k] = 0;
       }
-      if (kCols) {
+      if (qt) {
         const int pitch = (n_rb + 3) & ~3;
         st[int64_t(cb) * pitch + rb] = uint8_t(tile_byte);
         if (rb == n_rb - 1)
@@ -121,14 +137,14 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const T* __restrict_
     }
   }
 
-  if constexpr (kRows) {
+  if (q) {
     const int64_t Cp = int64_t(n_cb) * kBlock;
     const int pitch = (n_cb + 3) & ~3;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const int row = row0 + i;
       float inv = tile_inv;
-      if constexpr (!kTiles) {
+      if (!mat.tiles) {
         float m = 0.f;
 #pragma unroll
         for (int k = 0; k < 8; ++k) m = fmaxf(m, finite_abs(v[i][k]));
@@ -150,7 +166,7 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const T* __restrict_
     }
   }
 
-  if constexpr (kSums) {  // column sums of this 128-row block: rows in a thread, row groups in a wave, waves in order
+  if (mat.sums) {  // column sums of this 128-row block: rows in a thread, row groups in a wave, waves in order
     float sum[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
@@ -165,13 +181,13 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const T* __restrict_
       for (int k = 0; k < 8; ++k) red[wave][8 * j + k] = sum[k];
     __syncthreads();
     if (tid < kBlock && cb * kBlock + tid < C)
-      sums[int64_t(rb) * C + cb * kBlock + tid] = (red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid]);
+      mat.sums[int64_t(rb) * C + cb * kBlock + tid] = (red[0][tid] + red[1][tid]) + (red[2][tid] + red[3][tid]);
     __syncthreads();
   }
 
-  if constexpr (kCols) {
+  if (qt) {
     float inv[8];
-    if constexpr (kTiles) {
+    if (mat.tiles) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) inv[k] = tile_inv;
     } else {
@@ -223,69 +239,22 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const T* __restrict_
   }
 }
 
-template <typename Out>
-__global__ __launch_bounds__(kThreads) void fold_column_sums_kernel(const float* __restrict__ sums, int n_rb, int C,
-                                                                    Out* __restrict__ out, bool accumulate) {
-  // 64 columns per workgroup; wave w adds the blocks w, w + 4, ... and the four sums meet in LDS.
-  __shared__ float red[4][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int c = blockIdx.x * 64 + lane;
-  float a = 0.f;
-  if (c < C)
-    for (int b = wave; b < n_rb; b += 4) a += sums[int64_t(b) * C + c];
-  red[wave][lane] = a;
-  __syncthreads();
-  if (wave == 0 && c < C) {
-    a = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
-    if (accumulate) a += VecIO<Out>::load1(out + c);
-    VecIO<Out>::store1(out + c, a);
-  }
-}
-
-template <typename T, bool kVec>
-void launch_quantize(const T* x, int64_t ld, int R, int C, bool tiles, uint8_t* q, uint8_t* s, uint8_t* qt, uint8_t* st,
-                     float* sums, hipStream_t stream) {
-  const dim3 grid((unsigned)ceil_div(C, kBlock), (unsigned)ceil_div(R, kBlock)), block(kThreads);
-  auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, block, 0, stream, x, ld, R, C, q, s, qt, st, sums); };
-  if (tiles) {
-    if (q && qt) go(quantize_kernel<T, kVec, true, true, true, false>);
-    else if (q) go(quantize_kernel<T, kVec, true, false, true, false>);
-    else go(quantize_kernel<T, kVec, false, true, true, false>);
-  } else if (sums) {
-    if (q && qt) go(quantize_kernel<T, kVec, true, true, false, true>);
-    else if (q) go(quantize_kernel<T, kVec, true, false, false, true>);
-    else go(quantize_kernel<T, kVec, false, true, false, true>);
-  } else {
-    if (q && qt) go(quantize_kernel<T, kVec, true, true, false, false>);
-    else if (q) go(quantize_kernel<T, kVec, true, false, false, false>);
-    else go(quantize_kernel<T, kVec, false, true, false, false>);
-  }
-}
-
 }  // namespace
 
-void fp8_quantize(DType dtype, const void* x, int64_t ld, int R, int C, bool tiles, uint8_t* q, uint8_t* scale,
-                  uint8_t* qt, uint8_t* scale_t, float* column_sums, hipStream_t stream) {
+void fp8_quantize(DType dtype, const Fp8QuantProblem* problems, int n, hipStream_t stream) {
   const int size = dtype == kBF16 ? 2 : 4;
-  const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (ld * size) % 16 == 0;
-  if (dtype == kBF16) {
-    const auto* p = (const bf16_raw*)x;
-    if (vec) launch_quantize<bf16_raw, true>(p, ld, R, C, tiles, q, scale, qt, scale_t, column_sums, stream);
-    else launch_quantize<bf16_raw, false>(p, ld, R, C, tiles, q, scale, qt, scale_t, column_sums, stream);
-  } else {
-    const auto* p = (const float*)x;
-    if (vec) launch_quantize<float, true>(p, ld, R, C, tiles, q, scale, qt, scale_t, column_sums, stream);
-    else launch_quantize<float, false>(p, ld, R, C, tiles, q, scale, qt, scale_t, column_sums, stream);
+  Matrices all = {};
+  int64_t blocks = 0;
+  for (int i = 0; i < n; ++i) {
+    const Fp8QuantProblem& p = problems[i];
+    const int64_t b = ceil_div(p.C, kBlock) * ceil_div(p.R, kBlock);
+    const bool vec = reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && (p.ld * size) % 16 == 0;
+    all.m[i] = Matrix{p.x, p.ld, p.R, p.C, (int)b, vec, p.tiles, p.q, p.scale, p.qt, p.scale_t, p.column_sums};
+    blocks += b;
   }
-}
-
-void fp8_fold_column_sums(const float* sums, int n_blocks, int C, DType out_dtype, void* out, bool accumulate,
-                          hipStream_t stream) {
-  const dim3 grid((unsigned)ceil_div(C, 64)), block(kThreads);
-  if (out_dtype == kBF16)
-    hipLaunchKernelGGL(fold_column_sums_kernel<bf16_raw>, grid, block, 0, stream, sums, n_blocks, C, (bf16_raw*)out, accumulate);
-  else
-    hipLaunchKernelGGL(fold_column_sums_kernel<float>, grid, block, 0, stream, sums, n_blocks, C, (float*)out, accumulate);
+  const dim3 grid((unsigned)blocks), block(kThreads);
+  if (dtype == kBF16) hipLaunchKernelGGL(quantize_kernel<bf16_raw>, grid, block, 0, stream, all);
+  else hipLaunchKernelGGL(quantize_kernel<float>, grid, block, 0, stream, all);
 }
 
 }  // namespace pda

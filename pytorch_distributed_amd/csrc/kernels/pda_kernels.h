@@ -168,15 +168,21 @@ void gemm_fused(const void* X, int64_t ldx, const void* W, int64_t ldw, const vo
 // columns, transposed), or with `tiles` one scale per 128 x 128 tile (scale [ceil(R/128), Sc], scale_t
 // [ceil(C/128), Sr]). Cp / Rp: rounded up to 128, Sc / Sr: block counts rounded up to 4; all padding is
 // zeroed. Either output pair may be null. column_sums (without tiles): fp32 [ceil(R/128), C] partial sums of
-// x, folded in order by fp8_fold_column_sums into out [C].
-void fp8_quantize(DType dtype, const void* x, int64_t ld, int R, int C, bool tiles, uint8_t* q, uint8_t* scale,
-                  uint8_t* qt, uint8_t* scale_t, float* column_sums, hipStream_t stream);
-void fp8_fold_column_sums(const float* sums, int n_blocks, int C, DType out_dtype, void* out, bool accumulate,
-                          hipStream_t stream);
+// x. 1 <= n <= 3 non-empty matrices of one dtype share the launch.
+struct Fp8QuantProblem {
+  const void* x;
+  int64_t ld;
+  int R, C;
+  bool tiles;
+  uint8_t *q, *scale, *qt, *scale_t;
+  float* column_sums;
+};
+void fp8_quantize(DType dtype, const Fp8QuantProblem* problems, int n, hipStream_t stream);
 // out[M, N] = (out +) bias + x . w^T for such operands: `rows` rows of ld bytes (K of them read, K % 128 == 0),
 // scales at row (or row / 128 with `tiles`), ld_scale bytes a row (a multiple of 4, at least K / 128). out and
 // the bias are contiguous. fp8_gemm_plan chooses the tile and how often the contraction is cut; more than one
-// slice needs `partial`, fp32 [slices][M][N].
+// slice, or `accumulate`, needs `partial`, fp32 [slices][M][N], 16-byte aligned. 1 <= n <= 2 independent
+// products; `sums` (optional) folds the partial column sums of fp8_quantize into out [C] along with them.
 struct Fp8Operand {
   const void* q;
   const void* scale;
@@ -187,9 +193,26 @@ struct Fp8Operand {
 struct Fp8GemmPlan {
   int tile, slices, steps_per_slice;
 };
+struct Fp8GemmProblem {
+  Fp8Operand x, w;
+  int K;
+  const void* bias;
+  DType bias_dtype;
+  void* out;
+  DType out_dtype;
+  bool accumulate;
+  Fp8GemmPlan plan;
+  float* partial;
+};
+struct Fp8ColumnSums {
+  const float* partial;
+  int blocks, C;
+  void* out;
+  DType out_dtype;
+  bool accumulate;
+};
 Fp8GemmPlan fp8_gemm_plan(int M, int N, int K, DType out_dtype);
-void fp8_gemm(const Fp8Operand& x, const Fp8Operand& w, int K, const void* bias, DType bias_dtype, void* out,
-              DType out_dtype, bool accumulate, const Fp8GemmPlan& plan, float* partial, hipStream_t stream);
+void fp8_gemm(const Fp8GemmProblem* problems, int n, const Fp8ColumnSums* sums, hipStream_t stream);
 
 // ----------------------------------------------------------------- Embedding --
 // out[n, :] = wte[ids[n], :] (+ wpe[n mod T, :] when wpe != nullptr). d % (16 / sizeof(T)) == 0.

@@ -123,29 +123,6 @@ def causal_attention(qkv: torch.Tensor, num_heads: int, scale: float | None = No
     return attention_sdpa(qkv, num_heads, scale)
 
 
-def _packed(t: torch.Tensor) -> torch.Tensor:
-    """Contiguous and on a 16-byte boundary, as the kernels' vector loads need it."""
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
-class _WindowAttentionFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, qkv, num_heads, window, sinks, scale, dropout_p, seed):
-        qkv = _packed(qkv)
-        ctx.args = (num_heads, window, sinks, scale, dropout_p, seed)
-        out, lse = _ext.require().window_attention_forward(qkv, *ctx.args)
-        ctx.save_for_backward(qkv, out, lse)
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dout):
-        qkv, out, lse = ctx.saved_tensors
-        dqkv = _ext.require().window_attention_backward(qkv, out, _packed(dout), lse, *ctx.args)
-        return (dqkv,) + (None,) * 6
-
-
 def window_attention(qkv: torch.Tensor, num_heads: int, window: int, sinks: int = 0, scale: float | None = None,
                      dropout_p: float = 0.0, training: bool = False, seed: int | None = None) -> torch.Tensor:
     """:func:`causal_attention` inside a sliding window: query t sees the ``window`` keys ``t - window + 1 .. t``
@@ -181,4 +158,4 @@ def window_attention(qkv: torch.Tensor, num_heads: int, window: int, sinks: int 
         return window_attention(qkv.to(torch.bfloat16), num_heads, window, sinks, scale, p, training, seed).to(torch.float32)
     if p > 0.0:
         seed = _draw_seed() if seed is None else int(seed)
-    return _WindowAttentionFn.apply(qkv, num_heads, window, sinks, scale, p, seed if p > 0.0 else 0)
+    return _ext.require().window_attention(qkv, num_heads, window, sinks, scale, p, seed if p > 0.0 else 0)
