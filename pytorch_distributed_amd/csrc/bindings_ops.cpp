@@ -743,7 +743,7 @@ pda::Fp8Operand fp8_operand(const at::Tensor& q, const at::Tensor& scale, bool t
 struct Fp8Products {
   pda::Fp8GemmProblem problems[2];
   int n = 0;
-  std::vector<at::Tensor> partials;
+  at::TensorOptions partial_options;
 
   // out[M, N] = (out +) bias + x . w^T over K; `out` fresh in `dtype` unless given.
   at::Tensor add(const Fp8Pair& x, bool x_tiles, const Fp8Pair& w, bool w_tiles, int64_t K, const std::optional<at::Tensor>& bias,
@@ -773,17 +773,20 @@ struct Fp8Products {
       if (bias.has_value()) y.view({M, N}).add_(*bias);
       return y;
     }
-    const pda::Fp8GemmPlan plan = pda::fp8_gemm_plan((int)M, (int)N, (int)X.ld, out_dtype);
-    float* partial = nullptr;
-    if (plan.slices > 1 || accumulate) {
-      partials.push_back(at::empty({plan.slices, M, N}, x.q.options().dtype(at::kFloat)));
-      partial = partials.back().data_ptr<float>();
-    }
-    problems[n++] = {X, W, (int)X.ld, bias.has_value() ? bias->data_ptr() : nullptr, bias_dtype, y.data_ptr(), out_dtype, accumulate, plan, partial};
+    problems[n++] = {X, W, (int)X.ld, bias.has_value() ? bias->data_ptr() : nullptr, bias_dtype, y.data_ptr(), out_dtype, accumulate, {}, nullptr};
+    partial_options = x.q.options().dtype(at::kFloat);
     return y;
   }
   void run(const pda::Fp8ColumnSums* sums = nullptr) {
     if (n == 0 && !sums) return;
+    at::Tensor partials[2];
+    pda::fp8_gemm_plan(problems, n);
+    for (int i = 0; i < n; ++i) {
+      pda::Fp8GemmProblem& p = problems[i];
+      if (p.plan.slices == 1 && !p.accumulate) continue;
+      partials[i] = at::empty({p.plan.slices, p.x.rows, p.w.rows}, partial_options);
+      p.partial = partials[i].data_ptr<float>();
+    }
     pda::fp8_gemm(problems, n, sums, current_stream());
     check_launch("fp8_gemm");
   }

@@ -474,20 +474,60 @@ void launch(const Problems& P, hipStream_t stream) {
 
 }  // namespace
 
-Fp8GemmPlan fp8_gemm_plan(int M, int N, int K, DType out_dtype) {
-  Fp8GemmPlan p;
+// Which tile, and how many slices of the contraction: the smallest estimated time. The estimate is rounds of
+// workgroups over the chip's slots, in microseconds fitted to measurements of 12 shapes from 16 x 3840 x 1280 to
+// 8192 x 22016 x 4096 (most within 10 %). A stage of a 256 tile takes 0.72 with every compute unit busy (0.47
+// alone); of a 128 tile 0.20 alone, 0.29 with one workgroup per compute unit, 0.60 with two. What else a
+// workgroup costs (first loads, stores) is 10 and 3.3. So 8192 x 1280 x 5120 takes the 256 tile (160 of them: 65
+// against 77), 2048^3 the 128 tile (13 against 28). A slice's partial sums are written and read again at some
+// 4.5 TB/s and folded by a launch of 3: 1024 x 1024 x 8192 gains by four slices (33 -> 23), 2048^3 loses by two
+// (13 -> 31). The widened products have the 128 tile only, at 1.5 times its stage.
+static float plan_time(int tile, int64_t tasks, int steps, bool wide) {
+  const int64_t slots = tile == 256 ? 256 : 512;
+  auto round = [&](int64_t n) {
+    const float load = n / 256.f;
+    if (tile == 256) return 10.f + steps * (0.47f + 0.25f * load);
+    const float stage = load <= 1.f ? 0.20f + 0.09f * load : 0.29f + 0.31f * (load - 1.f);
+    return 3.3f + steps * stage * (wide ? 1.5f : 1.f);
+  };
+  const int64_t full = tasks / slots, rest = tasks % slots;
+  return (tile == 256 ? 4.f : 1.4f) + full * round(slots) + (rest ? round(rest) : 0.f);
+}
+
+static Fp8GemmPlan plan_for_tile(int tile, int M, int N, int K, bool wide, float* time) {
   const int steps = K / kStageK, groups = (steps + kGroupStages - 1) / kGroupStages;
-  const int64_t big = ceil_div(M, 256) * ceil_div(N, 256);
-  p.tile = big >= 192 && out_dtype == kBF16 ? 256 : 128;
-  const int64_t tiles = ceil_div(M, p.tile) * ceil_div(N, p.tile);
-  int slices = 1;
-  const int slots = p.tile == 256 ? 256 : 512;  // workgroups the chip runs at once
-  if (tiles < slots) slices = (int)(slots / tiles < groups ? slots / tiles : groups);
-  if (slices < 1) slices = 1;
-  const int per = (groups + slices - 1) / slices;
-  p.steps_per_slice = per * kGroupStages;
-  p.slices = (groups + per - 1) / per;
-  return p;
+  const int64_t tiles = ceil_div(M, tile) * ceil_div(N, tile);
+  Fp8GemmPlan best{tile, 1, groups * kGroupStages};
+  *time = plan_time(tile, tiles, steps, wide);
+  for (int slices = 2; slices <= groups && slices <= 16; ++slices) {
+    const int per = (groups + slices - 1) / slices;
+    const int real = (groups + per - 1) / per;  // slices that have any work
+    if (real != slices) continue;
+    const float t = plan_time(tile, tiles * slices, per * kGroupStages, wide) + 3.f + float(M) * N * (8.f * slices + 2.f) / 4.5e6f;
+    if (t < *time) {
+      *time = t;
+      best = Fp8GemmPlan{tile, slices, per * kGroupStages};
+    }
+  }
+  return best;
+}
+
+// Products that run together take the tile that is best for their sum, so that they share a launch.
+void fp8_gemm_plan(Fp8GemmProblem* problems, int n) {
+  Fp8GemmPlan plans[2][2];
+  float sum[2] = {0.f, 0.f};
+  bool wide = false;
+  for (int i = 0; i < n; ++i) {
+    Fp8GemmProblem& p = problems[i];
+    wide |= p.out_dtype == kF32;
+    for (int k = 0; k < 2; ++k) {
+      float t;
+      plans[k][i] = plan_for_tile(k ? 256 : 128, p.x.rows, p.w.rows, p.K, p.out_dtype == kF32, &t);
+      sum[k] += t;
+    }
+  }
+  const int k = !wide && sum[1] < sum[0];
+  for (int i = 0; i < n; ++i) problems[i].plan = plans[k][i];
 }
 
 void fp8_gemm(const Fp8GemmProblem* problems, int n, const Fp8ColumnSums* sums, hipStream_t stream) {
@@ -523,7 +563,8 @@ void fp8_gemm(const Fp8GemmProblem* problems, int n, const Fp8ColumnSums* sums, 
   };
   auto wide = [&](int i) { return problems[i].out_dtype == kF32; };
   if (n == 2 && problems[0].plan.tile == problems[1].plan.tile && wide(0) == wide(1)) {
-    go(ps[0], &ps[1], problems[0].plan.tile, wide(0));
+    const int longer = ps[1].steps_per_slice > ps[0].steps_per_slice;  // long tasks first: the short ones fill up
+    go(ps[longer], &ps[1 - longer], problems[0].plan.tile, wide(0));
   } else {
     for (int i = 0; i < n; ++i) go(ps[i], nullptr, problems[i].plan.tile, wide(i));
   }

@@ -211,7 +211,7 @@ struct Fp8ColumnSums {
   DType out_dtype;
   bool accumulate;
 };
-Fp8GemmPlan fp8_gemm_plan(int M, int N, int K, DType out_dtype);
+void fp8_gemm_plan(Fp8GemmProblem* problems, int n);  // sets their `plan` (out and partial may still be null)
 void fp8_gemm(const Fp8GemmProblem* problems, int n, const Fp8ColumnSums* sums, hipStream_t stream);
 
 // ----------------------------------------------------------------- Embedding --
