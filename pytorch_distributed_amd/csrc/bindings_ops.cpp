@@ -820,11 +820,12 @@ std::vector<at::Tensor> fp8_linear_forward(const at::Tensor& x, const at::Tensor
   Fp8Products products;
   std::optional<at::Tensor> b;
   if (bias.has_value()) b = bias->contiguous();
-  at::Tensor y = products.add(xr, false, wr, true, x2.size(1), b, x.scalar_type(), std::nullopt, false);
-  products.run();
+  // allocated in its final shape, not returned as a view: a following op may work on it in place (the rotary one does)
   std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = weight.size(0);
-  y = y.view(shape);
+  at::Tensor y = at::empty(shape, x.options());
+  products.add(xr, false, wr, true, x2.size(1), b, x.scalar_type(), y, false);
+  products.run();
   if (keep) return {y, xc.q, xc.scale};
   return {y};
 }

@@ -14,7 +14,7 @@ releases no longer define ``n_ctx``.
 from __future__ import annotations
 
 from dataclasses import asdict, dataclass, replace
-from typing import Any, Dict
+from typing import Any, Dict, Optional
 
 
 @dataclass
@@ -30,6 +30,12 @@ class GPT2Config:
     embd_pdrop: float = 0.1
     layer_norm_epsilon: float = 1e-5
     name: str = "gpt2"
+    # Not in the reference: operands of the blocks' linear layers ("bf16", or "fp8": 8-bit with block scales,
+    # ops.fp8_linear; embeddings and the LM head stay as they are), and attention inside a sliding window
+    # (None: all earlier keys) with the first `attention_sinks` keys always visible (ops.window_attention).
+    linear_precision: str = "bf16"
+    sliding_window: Optional[int] = None
+    attention_sinks: int = 0
 
     @property
     def n_positions(self) -> int:
@@ -59,6 +65,9 @@ class LlamaConfig:
     rope_theta: float = 10000.0
     tie_word_embeddings: bool = False
     name: str = "llama-7b"
+    linear_precision: str = "bf16"  # as in GPT2Config
+    sliding_window: Optional[int] = None
+    attention_sinks: int = 0
 
     @property
     def head_dim(self) -> int:
@@ -70,6 +79,18 @@ class LlamaConfig:
     def without_dropout(self) -> "LlamaConfig":
         """Llama-style models have no dropout; present so callers can treat both families alike."""
         return self
+
+
+def check_block_options(config) -> None:
+    """Refuses values of ``linear_precision`` / ``sliding_window`` / ``attention_sinks`` that mean nothing."""
+    if config.linear_precision not in ("bf16", "fp8"):
+        raise ValueError(f"linear_precision must be 'bf16' or 'fp8', got {config.linear_precision!r}")
+    if config.sliding_window is not None and int(config.sliding_window) < 1:
+        raise ValueError(f"sliding_window must be at least 1 (or None), got {config.sliding_window}")
+    if int(config.attention_sinks) < 0:
+        raise ValueError(f"attention_sinks must not be negative, got {config.attention_sinks}")
+    if config.attention_sinks and config.sliding_window is None:
+        raise ValueError("attention_sinks needs a sliding_window (without one every earlier key is visible)")
 
 
 _GPT2 = {
@@ -112,7 +133,10 @@ def normalize_gpt2_config(config) -> GPT2Config:
         attn_pdrop=getattr(config, "attn_pdrop", 0.1), resid_pdrop=getattr(config, "resid_pdrop", 0.1),
         embd_pdrop=getattr(config, "embd_pdrop", 0.1),
         layer_norm_epsilon=getattr(config, "layer_norm_epsilon", 1e-5),
-        name=getattr(config, "name_or_path", None) or "gpt2-custom")
+        name=getattr(config, "name_or_path", None) or "gpt2-custom",
+        linear_precision=getattr(config, "linear_precision", "bf16"),
+        sliding_window=getattr(config, "sliding_window", None),
+        attention_sinks=getattr(config, "attention_sinks", 0))
 
 
 def gpt2_param_count(cfg: GPT2Config) -> int:

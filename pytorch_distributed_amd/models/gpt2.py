@@ -40,9 +40,9 @@ import torch
 from torch import nn
 
 from .. import ops
-from ..ops.regen import NormRegen
+from ..ops.regen import GeluRegen, NormRegen
 from ..utils.recompute import recompute
-from .config import GPT2Config, get_config, normalize_gpt2_config
+from .config import check_block_options, GPT2Config, get_config, normalize_gpt2_config
 
 
 class MyGPT2Attention(nn.Module):
@@ -57,6 +57,9 @@ class MyGPT2Attention(nn.Module):
         self.c_attn = nn.Linear(self.embed_dim, 3 * self.embed_dim, bias=True)
         self.c_proj = nn.Linear(self.embed_dim, self.embed_dim, bias=True)
         self.attn_pdrop = float(config.attn_pdrop)
+        check_block_options(config)
+        self.linear = ops.fp8_linear if config.linear_precision == "fp8" else ops.linear
+        self.sliding_window, self.attention_sinks = config.sliding_window, config.attention_sinks
         self.resid_dropout = nn.Dropout(p=config.resid_pdrop)
 
     def forward(self, hidden_states: torch.Tensor, apply_dropout: bool = True, input_regen=None) -> torch.Tensor:
@@ -64,9 +67,13 @@ class MyGPT2Attention(nn.Module):
         into the next LayerNorm kernel). ``input_regen``: recipe that rebuilds ``hidden_states`` in
         backward (``ops.regen``), so that ``c_attn`` does not keep it."""
         # [B, T, 3d], consumed in place by the attention kernel
-        qkv = ops.linear(hidden_states, self.c_attn.weight, self.c_attn.bias, regen=input_regen)
-        ctx = ops.causal_attention(qkv, self.num_heads, dropout_p=self.attn_pdrop, training=self.training)
-        out = ops.linear(ctx, self.c_proj.weight, self.c_proj.bias)
+        qkv = self.linear(hidden_states, self.c_attn.weight, self.c_attn.bias, regen=input_regen)
+        if self.sliding_window is None:
+            ctx = ops.causal_attention(qkv, self.num_heads, dropout_p=self.attn_pdrop, training=self.training)
+        else:
+            ctx = ops.window_attention(qkv, self.num_heads, self.sliding_window, self.attention_sinks,
+                                       dropout_p=self.attn_pdrop, training=self.training)
+        out = self.linear(ctx, self.c_proj.weight, self.c_proj.bias)
         return self.resid_dropout(out) if apply_dropout else out
 
 
@@ -82,13 +89,20 @@ class MyGPT2MLP(nn.Module):
         self.c_fc = nn.Linear(self.embed_dim, 4 * self.embed_dim, bias=True)
         self.c_proj = nn.Linear(4 * self.embed_dim, self.embed_dim, bias=True)
         self.dropout = nn.Dropout(p=config.resid_pdrop)
+        check_block_options(config)
+        self.linear_precision = config.linear_precision
 
     def forward(self, hidden_states: torch.Tensor, apply_dropout: bool = True, input_regen=None,
                 regen_activation: bool = False) -> torch.Tensor:
         """``input_regen`` as in :class:`MyGPT2Attention`; ``regen_activation``: ``c_proj`` rebuilds
         ``gelu(u)`` from the kept ``u`` in backward instead of keeping it."""
-        out = ops.gelu_mlp(hidden_states, self.c_fc.weight, self.c_fc.bias, self.c_proj.weight, self.c_proj.bias,
-                           input_regen=input_regen, regen_activation=regen_activation)
+        if self.linear_precision == "fp8":
+            u = ops.fp8_linear(hidden_states, self.c_fc.weight, self.c_fc.bias, regen=input_regen)
+            out = ops.fp8_linear(ops.gelu_new(u), self.c_proj.weight, self.c_proj.bias,
+                                 regen=GeluRegen(u) if regen_activation else None)
+        else:
+            out = ops.gelu_mlp(hidden_states, self.c_fc.weight, self.c_fc.bias, self.c_proj.weight, self.c_proj.bias,
+                               input_regen=input_regen, regen_activation=regen_activation)
         return self.dropout(out) if apply_dropout else out
 
 

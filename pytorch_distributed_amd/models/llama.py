@@ -20,7 +20,7 @@ from torch import nn
 from .. import _ext, ops
 from ..ops.regen import NormRegen, SwigluRegen
 from ..utils.recompute import recompute
-from .config import LlamaConfig, get_config
+from .config import LlamaConfig, check_block_options, get_config
 
 
 class RMSNorm(nn.Module):
@@ -96,23 +96,32 @@ class LlamaAttention(nn.Module):
         super().__init__()
         self.num_heads = config.n_head
         self.head_dim = config.head_dim
+        check_block_options(config)
+        self.linear = ops.fp8_linear if config.linear_precision == "fp8" else ops.linear
+        self.sliding_window, self.attention_sinks = config.sliding_window, config.attention_sinks
         self.wqkv = nn.Linear(config.n_embd, 3 * config.n_embd, bias=False)
         self.c_proj = nn.Linear(config.n_embd, config.n_embd, bias=False)
 
     def forward(self, x, cos, sin, input_regen=None):
-        qkv = _RopePacked.apply(ops.linear(x, self.wqkv.weight, regen=input_regen), cos, sin, self.num_heads)
-        return ops.linear(ops.causal_attention(qkv, self.num_heads), self.c_proj.weight)
+        qkv = _RopePacked.apply(self.linear(x, self.wqkv.weight, regen=input_regen), cos, sin, self.num_heads)
+        if self.sliding_window is None:
+            ctx = ops.causal_attention(qkv, self.num_heads)
+        else:
+            ctx = ops.window_attention(qkv, self.num_heads, self.sliding_window, self.attention_sinks)
+        return self.linear(ctx, self.c_proj.weight)
 
 
 class LlamaMLP(nn.Module):
     def __init__(self, config: LlamaConfig):
         super().__init__()
+        check_block_options(config)
+        self.linear = ops.fp8_linear if config.linear_precision == "fp8" else ops.linear
         self.gate_up = nn.Linear(config.n_embd, 2 * config.intermediate_size, bias=False)
         self.down = nn.Linear(config.intermediate_size, config.n_embd, bias=False)
 
     def forward(self, x, input_regen=None, regen_activation: bool = False):
-        gu = ops.linear(x, self.gate_up.weight, regen=input_regen)
-        return ops.linear(ops.swiglu(gu), self.down.weight, regen=SwigluRegen(gu) if regen_activation else None)
+        gu = self.linear(x, self.gate_up.weight, regen=input_regen)
+        return self.linear(ops.swiglu(gu), self.down.weight, regen=SwigluRegen(gu) if regen_activation else None)
 
 
 class LlamaBlock(nn.Module):

@@ -67,6 +67,13 @@ def add_common_args(ap: argparse.ArgumentParser) -> argparse.ArgumentParser:
                     help="auto | off | all | N: run N of the loader's micro-batches as one forward / backward pass "
                          "(same optimizer step up to summation order, larger GEMMs, fewer collectives); auto = as "
                          "many as the memory left after the first window holds (GPU only)")
+    ap.add_argument("--linear-precision", choices=["bf16", "fp8"], default="bf16",
+                    help="operands of the blocks' linear layers: fp8 = e4m3 with a scale per block of 128 in all three "
+                         "products of a step (the LM head, the embeddings and the optimizer stay as they are)")
+    ap.add_argument("--sliding-window", type=int, default=None,
+                    help="attention sees the last N keys only (default: all earlier ones)")
+    ap.add_argument("--attention-sinks", type=int, default=0,
+                    help="with --sliding-window: the first N keys stay visible to every query")
     return ap
 
 
@@ -99,6 +106,9 @@ def build_model(args, device, dtype):
     cfg = get_config(args.model)
     if hasattr(cfg, "attn_pdrop") and args.dropout is not None:
         cfg.attn_pdrop = cfg.resid_pdrop = cfg.embd_pdrop = args.dropout
+    cfg.linear_precision = getattr(args, "linear_precision", "bf16")
+    cfg.sliding_window = getattr(args, "sliding_window", None)
+    cfg.attention_sinks = getattr(args, "attention_sinks", 0)
     torch.manual_seed(args.seed)
     if torch.cuda.is_available():
         torch.cuda.manual_seed(args.seed)

@@ -3,7 +3,7 @@
 Convention: training FLOPs per token = ``6 * N_mm + 12 * L * d * T`` where ``N_mm`` is
 the number of matmul weights (every Linear weight incl. the tied LM head; embeddings
 tables other than the head, biases and norms excluded), the attention term is not
-discounted for causality, and recomputation is not counted (model FLOPs, not hardware
+discounted for causality (under a sliding window ``T`` is at most the window plus its sinks), and recomputation is not counted (model FLOPs, not hardware
 FLOPs). MFU divides by the MI355X dense bf16 peak, ``MI355X_PEAK_BF16_FLOPS``.
 """
 from __future__ import annotations
@@ -23,6 +23,8 @@ def model_flops_per_token(model, seq_len: int) -> float:
     cfg = getattr(model, "config", None)
     if cfg is None:
         return 0.0
+    if getattr(cfg, "sliding_window", None) is not None:
+        seq_len = min(seq_len, cfg.sliding_window + cfg.attention_sinks)
     if hasattr(cfg, "intermediate_size"):  # Llama-style: 4 d^2 + 3 d f per layer, untied head
         n_mm = cfg.n_layer * (4 * cfg.n_embd ** 2 + 3 * cfg.n_embd * cfg.intermediate_size) \
             + cfg.n_embd * cfg.vocab_size
