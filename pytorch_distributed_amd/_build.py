@@ -32,6 +32,9 @@ REPO = PKG_DIR.parent
 OBJ_DIR = REPO / "build" / "obj"
 TARGET = PKG_DIR / "_C.so"
 ARCH = "gfx950"
+# Sources with flags of their own. attention_window*.hip: matrix results in ordinary registers; in accumulator
+# registers every score would be copied across before the vector unit can use it.
+EXTRA_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for name in ("attention_window.hip", "attention_window_dkv.hip")}
 ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 
 
@@ -111,7 +114,7 @@ def build(force: bool = False, verbose: bool = False, sanitize: bool = False) ->
         target.parent.mkdir(parents=True, exist_ok=True)
 
     jobs = int(os.environ.get("MAX_JOBS", "0")) or min(8, os.cpu_count() or 1)
-    tasks = [(s, [hipcc], hip_flags, kernel_hdrs) for s in kernel_srcs]
+    tasks = [(s, [hipcc], hip_flags + EXTRA_FLAGS.get(s.name, []), kernel_hdrs) for s in kernel_srcs]
     tasks += [(s, [cxx], host_flags, host_hdrs) for s in host_srcs]
     with ThreadPoolExecutor(max_workers=jobs) as pool:
         results = list(pool.map(lambda t: _compile(t[0], t[1], t[2], t[3], force, verbose), tasks))

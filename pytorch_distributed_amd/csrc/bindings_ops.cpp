@@ -382,49 +382,62 @@ at::Tensor packed16(const at::Tensor& t) {
   return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
 }
 
+// {out, out_rest, neg_lse}; out_rest (only with `for_backward`) and neg_lse are the backward's.
 std::vector<at::Tensor> window_attention_forward(const at::Tensor& qkv, int64_t num_heads, int64_t window, int64_t sinks,
-                                                 double softmax_scale, double dropout_p, uint64_t seed) {
+                                                 double softmax_scale, double dropout_p, uint64_t seed, bool for_backward) {
   const WindowShape w = check_window(qkv, num_heads, window, sinks, dropout_p);
   const c10::DeviceGuard guard(qkv.device());
   at::Tensor out = at::empty({w.B, w.T, w.H * w.D}, qkv.options());
-  at::Tensor lse = at::empty({w.B, w.H, w.T}, qkv.options().dtype(at::kFloat));
-  pda::window_attention_forward(qkv.data_ptr(), out.data_ptr(), lse.data_ptr<float>(), (int)w.B, (int)w.T, (int)w.H, (int)w.D,
-                                (int)w.window, (int)w.sinks, (float)softmax_scale, (float)dropout_p, seed, current_stream());
+  at::Tensor rest;
+  if (for_backward) rest = at::empty(out.sizes(), qkv.options().dtype(at::kByte));
+  at::Tensor neg_lse = at::empty({w.B, w.H, w.T}, qkv.options().dtype(at::kFloat));
+  pda::window_attention_forward(qkv.data_ptr(), out.data_ptr(), for_backward ? rest.data_ptr() : nullptr, neg_lse.data_ptr<float>(),
+                                (int)w.B, (int)w.T, (int)w.H, (int)w.D, (int)w.window, (int)w.sinks, (float)softmax_scale,
+                                (float)dropout_p, seed, current_stream());
   check_launch("window_attention_forward");
-  return {out, lse};
+  return {out, rest, neg_lse};
 }
 
-at::Tensor window_attention_backward(const at::Tensor& qkv, const at::Tensor& out, const at::Tensor& dout, const at::Tensor& lse,
-                                     int64_t num_heads, int64_t window, int64_t sinks, double softmax_scale, double dropout_p,
-                                     uint64_t seed) {
+at::Tensor window_attention_backward(const at::Tensor& qkv, const at::Tensor& out, const at::Tensor& out_rest, const at::Tensor& dout,
+                                     const at::Tensor& neg_lse, int64_t num_heads, int64_t window, int64_t sinks, double softmax_scale,
+                                     double dropout_p, uint64_t seed) {
   const WindowShape w = check_window(qkv, num_heads, window, sinks, dropout_p);
   check_gpu(out, "out");
+  check_gpu(out_rest, "out_rest");
   check_gpu(dout, "dout");
-  check_gpu(lse, "lse");
-  TORCH_CHECK(out.scalar_type() == at::kBFloat16 && dout.scalar_type() == at::kBFloat16 && lse.scalar_type() == at::kFloat,
+  check_gpu(neg_lse, "neg_lse");
+  TORCH_CHECK(out.scalar_type() == at::kBFloat16 && dout.scalar_type() == at::kBFloat16 && out_rest.scalar_type() == at::kByte &&
+                  neg_lse.scalar_type() == at::kFloat,
               "window attention backward: dtype mismatch");
-  TORCH_CHECK(out.numel() == w.B * w.T * w.H * w.D && dout.numel() == out.numel() && lse.numel() == w.B * w.H * w.T,
+  TORCH_CHECK(out.numel() == w.B * w.T * w.H * w.D && dout.numel() == out.numel() && out_rest.numel() == out.numel() &&
+                  neg_lse.numel() == w.B * w.H * w.T,
               "window attention backward: shape mismatch");
-  TORCH_CHECK(out.device() == qkv.device() && dout.device() == qkv.device() && lse.device() == qkv.device(),
+  TORCH_CHECK(out.device() == qkv.device() && dout.device() == qkv.device() && neg_lse.device() == qkv.device() &&
+                  out_rest.device() == qkv.device(),
               "window attention backward: tensors on different devices");
   const c10::DeviceGuard guard(qkv.device());
   at::Tensor dqkv = at::empty_like(qkv);
-  at::Tensor delta = at::empty_like(lse);
+  at::Tensor neg_delta = at::empty_like(neg_lse);
   const size_t bytes = pda::window_attention_backward_workspace_bytes((int)w.B, (int)w.T, (int)w.H, (int)w.D, (int)w.window, (int)w.sinks);
-  at::Tensor workspace = at::empty({(int64_t)bytes}, qkv.options().dtype(at::kByte));
-  pda::window_attention_backward(qkv.data_ptr(), out.data_ptr(), dout.data_ptr(), lse.data_ptr<float>(), delta.data_ptr<float>(),
-                                 dqkv.data_ptr(), bytes ? workspace.data_ptr() : nullptr, (int)w.B, (int)w.T, (int)w.H, (int)w.D,
-                                 (int)w.window, (int)w.sinks, (float)softmax_scale, (float)dropout_p, seed, current_stream());
+  at::Tensor workspace;
+  if (bytes) workspace = at::empty({(int64_t)bytes}, qkv.options().dtype(at::kByte));
+  pda::window_attention_dq(qkv.data_ptr(), out.data_ptr(), out_rest.data_ptr(), dout.data_ptr(), neg_lse.data_ptr<float>(),
+                           neg_delta.data_ptr<float>(), dqkv.data_ptr(), (int)w.B, (int)w.T, (int)w.H, (int)w.D, (int)w.window,
+                           (int)w.sinks, (float)softmax_scale, (float)dropout_p, seed, current_stream());
+  pda::window_attention_dkv(qkv.data_ptr(), dout.data_ptr(), neg_lse.data_ptr<float>(), neg_delta.data_ptr<float>(), dqkv.data_ptr(),
+                            bytes ? workspace.data_ptr() : nullptr, (int)w.B, (int)w.T, (int)w.H, (int)w.D, (int)w.window,
+                            (int)w.sinks, (float)softmax_scale, (float)dropout_p, seed, current_stream());
   check_launch("window_attention_backward");
   return dqkv;
 }
 
 struct WindowAttentionFn : public torch::autograd::Function<WindowAttentionFn> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& qkv, int64_t num_heads, int64_t window,
-                            int64_t sinks, double softmax_scale, double dropout_p, int64_t seed) {
+                            int64_t sinks, double softmax_scale, double dropout_p, int64_t seed, bool for_backward) {
     const at::Tensor packed = packed16(qkv);
-    auto got = window_attention_forward(packed, num_heads, window, sinks, softmax_scale, dropout_p, (uint64_t)seed);
-    ctx->save_for_backward({packed, got[0], got[1]});
+    auto got = window_attention_forward(packed, num_heads, window, sinks, softmax_scale, dropout_p, (uint64_t)seed, for_backward);
+    if (!for_backward) return got[0];
+    ctx->save_for_backward({packed, got[0], got[1], got[2]});
     auto& d = ctx->saved_data;
     d["args"] = std::vector<int64_t>{num_heads, window, sinks, seed};
     d["floats"] = std::vector<double>{softmax_scale, dropout_p};
@@ -435,15 +448,16 @@ struct WindowAttentionFn : public torch::autograd::Function<WindowAttentionFn> {
     const auto saved = ctx->get_saved_variables();
     const auto i = ctx->saved_data["args"].toIntVector();
     const auto f = ctx->saved_data["floats"].toDoubleVector();
-    at::Tensor dqkv = window_attention_backward(saved[0], saved[1], packed16(grads[0]), saved[2], i[0], i[1], i[2], f[0], f[1], (uint64_t)i[3]);
+    at::Tensor dqkv = window_attention_backward(saved[0], saved[1], saved[2], packed16(grads[0]), saved[3], i[0], i[1], i[2], f[0], f[1], (uint64_t)i[3]);
     const at::Tensor none;
-    return {dqkv, none, none, none, none, none, none};
+    return {dqkv, none, none, none, none, none, none, none};
   }
 };
 
 at::Tensor window_attention(const at::Tensor& qkv, int64_t num_heads, int64_t window, int64_t sinks, double softmax_scale,
                             double dropout_p, int64_t seed) {
-  return WindowAttentionFn::apply(qkv, num_heads, window, sinks, softmax_scale, dropout_p, seed);
+  return WindowAttentionFn::apply(qkv, num_heads, window, sinks, softmax_scale, dropout_p, seed,
+                                  at::GradMode::is_enabled() && qkv.requires_grad());
 }
 
 // keep[B, H, T, T] (bool): the attention-dropout mask the kernels apply for (dropout_p, seed).
@@ -1098,8 +1112,9 @@ void bind_ops(py::module_& m) {
   m.def("window_attention", &window_attention, py::arg("qkv"), py::arg("num_heads"), py::arg("window"), py::arg("sinks"),
         py::arg("softmax_scale"), py::arg("dropout_p"), py::arg("seed"));
   m.def("window_attention_forward", &window_attention_forward, py::arg("qkv"), py::arg("num_heads"), py::arg("window"),
-        py::arg("sinks"), py::arg("softmax_scale"), py::arg("dropout_p"), py::arg("seed"));
-  m.def("window_attention_backward", &window_attention_backward, py::arg("qkv"), py::arg("out"), py::arg("dout"), py::arg("lse"),
+        py::arg("sinks"), py::arg("softmax_scale"), py::arg("dropout_p"), py::arg("seed"), py::arg("for_backward") = false);
+  m.def("window_attention_backward", &window_attention_backward, py::arg("qkv"), py::arg("out"), py::arg("out_rest"),
+        py::arg("dout"), py::arg("neg_lse"),
         py::arg("num_heads"), py::arg("window"), py::arg("sinks"), py::arg("softmax_scale"), py::arg("dropout_p"), py::arg("seed"));
   m.def("attention_dropout_mask", &attention_dropout_mask, py::arg("B"), py::arg("H"), py::arg("T"),
         py::arg("dropout_p"), py::arg("seed"), py::arg("device"));

@@ -102,14 +102,19 @@ void attention_backward(const void* qkv, const void* out, const void* dout, cons
 void attention_dropout_mask(uint8_t* keep, int B, int T, int H, float dropout_p, uint64_t seed, hipStream_t stream);
 
 // The same inside a sliding window with sinks: query t sees keys s <= t with t - s < window or s < sinks
-// (1 <= window <= T, 0 <= sinks <= T). lse is in log2 units and goes back to the backward as it came. The
-// backward's workspace may be null where its size is 0.
-void window_attention_forward(const void* qkv, void* out, float* lse, int B, int T, int H, int D, int window, int sinks,
-                              float softmax_scale, float dropout_p, uint64_t seed, hipStream_t stream);
+// (1 <= window <= T, 0 <= sinks <= T). neg_lse (fp32 [B, H, T]) and out_rest (bytes, out's shape: what bf16 drops of
+// it) go back to the backward as they came; out_rest may be null in a forward without one. neg_delta: fp32
+// [B, H, T] scratch. The backward's workspace may be null where its size is 0.
+void window_attention_forward(const void* qkv, void* out, void* out_rest, float* neg_lse, int B, int T, int H, int D, int window,
+                              int sinks, float softmax_scale, float dropout_p, uint64_t seed, hipStream_t stream);
 size_t window_attention_backward_workspace_bytes(int B, int T, int H, int D, int window, int sinks);
-void window_attention_backward(const void* qkv, const void* out, const void* dout, const float* lse, float* delta,
-                               void* dqkv, void* workspace, int B, int T, int H, int D, int window, int sinks,
-                               float softmax_scale, float dropout_p, uint64_t seed, hipStream_t stream);
+// dq, then dkv (which takes neg_delta from it).
+void window_attention_dq(const void* qkv, const void* out, const void* out_rest, const void* dout, const float* neg_lse,
+                         float* neg_delta, void* dqkv, int B, int T, int H, int D, int window, int sinks, float softmax_scale,
+                         float dropout_p, uint64_t seed, hipStream_t stream);
+void window_attention_dkv(const void* qkv, const void* dout, const float* neg_lse, const float* neg_delta, void* dqkv,
+                          void* workspace, int B, int T, int H, int D, int window, int sinks, float softmax_scale, float dropout_p,
+                          uint64_t seed, hipStream_t stream);
 
 // ------------------------------------------------------------------- Rotary --
 // Rotates the Q and K thirds of a packed [B, T, 3, H, D] activation (rotate-half pairing) by

@@ -150,8 +150,8 @@ def window_attention(qkv: torch.Tensor, num_heads: int, window: int, sinks: int 
     if D not in (64, 128) or qkv.dtype not in (torch.bfloat16, torch.float32):
         raise NotImplementedError(f"window_attention on the GPU: head size {D} / dtype {qkv.dtype} has no kernel "
                                   "(head sizes 64 and 128; bf16, or fp32 computed through bf16 MFMA inputs)")
-    if scale <= 0.0:
-        raise ValueError(f"window_attention: the kernels take a positive scale, got {scale}")
+    if not 1e-20 <= scale <= 1e20:
+        raise ValueError(f"window_attention: the kernels take a positive scale between 1e-20 and 1e20, got {scale}")
     if B * T == 0:
         return qkv[..., : width // 3] * 0
     if qkv.dtype == torch.float32:  # fp32 storage: bf16 MFMA inputs, fp32 accumulation, widened result
