@@ -81,13 +81,6 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
   const bool wave_active = q0 < T;
   const KeyTiles tiles(s, qt * kBM, min(qt * kBM + kBM, T) - 1);
 
-  bf16x8 qf[kKSteps];
-#pragma unroll
-  for (int ks = 0; ks < kKSteps; ++ks)
-    qf[ks] = *reinterpret_cast<const bf16x8*>(q_base + int64_t(q_ld) * tok_stride + 16 * ks + 8 * h);
-  // Q has arrived here, not at its first use inside the loop, where the wait would include the next tile
-#pragma unroll
-  for (int ks = 0; ks < kKSteps; ++ks) asm volatile("" ::"v"(__builtin_bit_cast(u32x4, qf[ks])));
   TileLoader<D> loader;
   loader.init(tok_stride, wave, lane);
   auto fetch = [&](int i) {
@@ -96,6 +89,14 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
     loader.load(v_base, tiles[i] * kBN, T - 1, buf + kTileBytes, wave, lane);
   };
   fetch(0);
+  bf16x8 qf[kKSteps];
+#pragma unroll
+  for (int ks = 0; ks < kKSteps; ++ks)
+    qf[ks] = *reinterpret_cast<const bf16x8*>(q_base + int64_t(q_ld) * tok_stride + 16 * ks + 8 * h);
+  // Q arrives here, beside the first tile, not at its first use inside the loop, where the wait would include the
+  // next tile
+#pragma unroll
+  for (int ks = 0; ks < kKSteps; ++ks) asm volatile("" ::"v"(__builtin_bit_cast(u32x4, qf[ks])));
   TileAddr<D> at;
   at.init(lds_addr(smem), lane);
 
@@ -269,6 +270,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
     loader.load(k_base, tiles[i] * kBN, T - 1, buf, wave, lane);
     loader.load(v_base, tiles[i] * kBN, T - 1, buf + kTileBytes, wave, lane);
   };
+  fetch(0);
   bf16x8 qf[kKSteps], dof[kKSteps];
   float dpart = 0.f;
   {
@@ -288,8 +290,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
   const float delta = lane_pair_sum(dpart);
   const float neg_lse = neg_lse_in[int64_t(bh) * T + q_ld];
   if (h == 0 && q_row < T) neg_delta_out[int64_t(bh) * T + q_row] = -delta;
-  asm volatile("" ::"v"(neg_lse), "v"(delta));  // arrived before the first tile is on its way
-  fetch(0);
+  asm volatile("" ::"v"(neg_lse), "v"(delta));  // arrived here, not inside the loop
+#pragma unroll
+  for (int ks = 0; ks < kKSteps; ++ks) asm volatile("" ::"v"(__builtin_bit_cast(u32x4, qf[ks])));
   const float c = s.scale * kLog2e;
   TileAddr<D> at;
   at.init(lds_addr(smem), lane);

@@ -124,18 +124,6 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
   }
   const float c = s.scale * kLog2e;
 
-  bf16x8 kf[kKSteps], vf[kKSteps];
-#pragma unroll
-  for (int ks = 0; ks < kKSteps; ++ks) {
-    kf[ks] = *reinterpret_cast<const bf16x8*>(k_base + int64_t(key_ld) * tok_stride + 16 * ks + 8 * h);
-    vf[ks] = *reinterpret_cast<const bf16x8*>(v_base + int64_t(key_ld) * tok_stride + 16 * ks + 8 * h);
-  }
-  // K and V have arrived here, not at their first use inside the loop
-#pragma unroll
-  for (int ks = 0; ks < kKSteps; ++ks) {
-    asm volatile("" ::"v"(__builtin_bit_cast(u32x4, kf[ks])));
-    asm volatile("" ::"v"(__builtin_bit_cast(u32x4, vf[ks])));
-  }
   TileLoader<D> q_loader, do_loader;
   q_loader.init(tok_stride, wave, lane);
   do_loader.init(o_stride, wave, lane);
@@ -150,6 +138,19 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
       __builtin_amdgcn_global_load_lds((global_ptr_t*)src, (lds_ptr_t*)(row_smem + buf * 512 + wave * 256), 4, 0, 0);
     }
   };
+  if constexpr (!kFar) fetch(first_tile, 0);
+  bf16x8 kf[kKSteps], vf[kKSteps];
+#pragma unroll
+  for (int ks = 0; ks < kKSteps; ++ks) {
+    kf[ks] = *reinterpret_cast<const bf16x8*>(k_base + int64_t(key_ld) * tok_stride + 16 * ks + 8 * h);
+    vf[ks] = *reinterpret_cast<const bf16x8*>(v_base + int64_t(key_ld) * tok_stride + 16 * ks + 8 * h);
+  }
+  // K and V arrive here, beside the first tile, not at their first use inside the loop
+#pragma unroll
+  for (int ks = 0; ks < kKSteps; ++ks) {
+    asm volatile("" ::"v"(__builtin_bit_cast(u32x4, kf[ks])));
+    asm volatile("" ::"v"(__builtin_bit_cast(u32x4, vf[ks])));
+  }
   TileAddr<D> at;
   at.init(lds_addr(smem), lane);
   unsigned row_at = lds_addr(row_smem) + 16u * (unsigned)h;  // row constants 4 h ..; 8 rows further: + 32 bytes
@@ -361,7 +362,6 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
     return;
   }
 
-  fetch(first_tile, 0);
   for (int j = first_tile; j < end_tile; ++j) {
     const int buf = (j - first_tile) & 1;
     next_tile_ready();
