@@ -54,13 +54,13 @@ __device__ __forceinline__ void unpack_rest(u32x2 w, float (&out)[8]) {
 
 // ======================================================================= forward
 template <int D, bool kDrop>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 64 && !kDrop ? 3 : 2))) void window_fwd_kernel(
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 64 ? (kDrop ? 3 : 4) : 2))) void window_fwd_kernel(
     const bf16_raw* __restrict__ qkv, bf16_raw* __restrict__ out, uint8_t* __restrict__ out_rest,
     float* __restrict__ neg_lse_out, Shape s, DropoutParams drop) {
   constexpr int kKSteps = D / 16;
   constexpr int kDBlocks = D / 32;
   constexpr int kTileBytes = kBN * D * 2;
-  constexpr int kAhead = 6, kAheadV = 3;  // row reads / transposed fragments in flight
+  constexpr int kAhead = D == 64 ? 4 : 6, kAheadV = D == 64 ? 2 : 3;  // row reads / transposed fragments in flight
   extern __shared__ __attribute__((aligned(16))) char smem[];  // [2 buffers][K tile | V tile]
 
   const int lane = threadIdx.x & 63;
