@@ -8,12 +8,18 @@
 //
 // Structure. A workgroup of 4 waves (2 x 2) owns a square output tile, each wave a quarter as kWB x kWB
 // blocks of 32 x 32. A pipeline stage is 64 values of the contraction: [tile rows][64 bytes] of each
-// operand, moved global -> LDS by global_load_lds into a ring of four. The body of stage t
+// operand, moved global -> LDS by buffer loads into a ring of four. The body of stage t
 //   * waits until stage t + 1 has landed (counted: two younger stages stay in flight) and meets the
 //     other waves, who by then have read stage t out of LDS;
 //   * issues the products of stage t from registers, and between them the LDS reads of stage t + 1 and
 //     the loads of stage t + 4 into the slot that stage t has left.
 // One barrier per 16 matrix instructions (1,024 matrix cycles) of a wave at kWB = 4.
+// 256 tile (one workgroup per compute unit): a workgroup takes several tiles, and the stages run on across
+// them: while a tile is rounded and stored, the next one's first four stages are on their way. Measured against
+// a workgroup per tile: 8192 x 5120 x 1280 (640 tiles) 84 -> 72 us, 8192 x 22016 x 4096 (2,752) 665 -> 591.
+// What bounds it: the matrix pipes at the clock that the power leaves. 8192 x 22016 x 4096 runs at 2,500 TFLOP/s
+// (a library product of 8192^3 at 2,593); short contractions pay some 3 us a tile for the epilogue.
+// 128 tile: two workgroups per compute unit cover each other's first loads and epilogue.
 // The 16-byte chunk index of an LDS row is XOR-permuted with bits 2-3 of the row (on the source address:
 // the destination of such a load is linear), which makes the ds_read_b128 of 32 rows conflict free. A
 // lane's 32 bytes are chunks h and 2 + h of the row: the same order for both operands, and inside one
@@ -25,10 +31,11 @@
 // bits: measured (random e4m3 operands) up to 1.3e-4 of sum |x w|, 5e-5 in norm, whatever the contraction's
 // length. Next to a bf16 result's rounding (1.7e-3) that is nothing; an fp32 result is computed with kWide
 // instead: fragments widened to bf16 on the way to v_mfma_f32_32x32x16_bf16, scale included (exact), whose
-// sums are good to 6e-8, at half the matrix rate.
+// sums are good to 6e-8, at half the matrix rate (1003 x 1601 x 777: 14.4 us).
 //
 // Few output tiles (weight gradients, few tokens): the contraction is cut into slices of whole 512-value
 // scale groups, fp32 partial tiles are folded in slice order by a second kernel (deterministic).
+#include <algorithm>
 #include <type_traits>
 
 #include "attention_common.h"
@@ -43,6 +50,7 @@ constexpr int kThreads = 256;
 constexpr int kStages = 4;
 constexpr int kStageK = 64;                 // values (bytes) of the contraction per stage
 constexpr int kGroupStages = 8;             // stages whose scales are fetched together: 4 blocks of 128, a dword a row
+constexpr int kSlots = 256;                 // workgroups of the 256 tile at once: one per compute unit
 constexpr int kGroupM = 4;                  // token tiles walked together by consecutive tasks
 
 __device__ __forceinline__ unsigned lds_addr(const char* p) {
@@ -106,110 +114,168 @@ struct Problem {
   int steps, steps_per_slice, tasks;
 };
 
-// Up to two independent products in one launch (the two gradients of a layer): problem 1's workgroups follow
-// problem 0's, padded to a multiple of 8 so that both see their XCD as blockIdx % 8.
+// Up to two independent products in one launch (the two gradients of a layer): problem 1's tasks follow problem 0's.
 struct Problems {
   Problem p[2];
 };
 
+// The output tile and the slice of the contraction of one task.
+struct Place {
+  int which, slice, m0, n0, first, n_steps;  // which < 0: none
+};
+
+// Task `round` of workgroup `w` of `grid`: a round is the next `grid` tasks, every other one is dealt backwards
+// (whoever had a long task then gets a short one). Within a round, and within a problem, the 8 XCDs get contiguous
+// ranges; consecutive tasks walk kGroupM token tiles x all feature tiles, so an XCD's workgroups share operand
+// rows in its L2.
+template <int kTile>
+__device__ __forceinline__ Place place_of(const Problems& P, int w, int grid, int round) {
+  const int base = round * grid, left = P.p[0].tasks + P.p[1].tasks - base;
+  const int count = min(grid, left);
+  if (round & 1) w = grid - 1 - w;
+  Place at;
+  at.which = -1;
+  if (w >= count) return at;
+  const int c0 = max(min(P.p[0].tasks - base, count), 0);
+  const bool second = w >= c0;
+  const int n = second ? count - c0 : c0, j = second ? w - c0 : w;
+  const int q8 = n / 8, r8 = n % 8, x = j % 8;
+  const int task = base + (second ? c0 - P.p[0].tasks : 0) + (x < r8 ? x * (q8 + 1) : r8 * (q8 + 1) + (x - r8) * q8) + j / 8;
+  const Problem& pr = P.p[second];
+  const int tiles_m = (pr.x.rows + kTile - 1) / kTile, tiles_n = (pr.w.rows + kTile - 1) / kTile;
+  const int n_tiles = tiles_m * tiles_n;
+  const int slice = task / n_tiles;
+  const int tile = task - slice * n_tiles;
+  const int group = tile / (kGroupM * tiles_n);
+  const int in_group = tile - group * (kGroupM * tiles_n);
+  const int group_rows = min(kGroupM, tiles_m - group * kGroupM);
+  at.which = second;
+  at.slice = slice;
+  at.m0 = (group * kGroupM + in_group % group_rows) * kTile;
+  at.n0 = (in_group / group_rows) * kTile;
+  at.first = slice * pr.steps_per_slice;  // a multiple of kGroupStages
+  at.n_steps = min(pr.steps_per_slice, pr.steps - at.first);
+  return at;
+}
+
+constexpr int kScaleRing = 4;  // scale groups in LDS: loads run at most 4 stages ahead, at least 2 stages (one group) a tile
+constexpr int kBiasRing = 4;   // likewise of tiles
+constexpr int kWaveStage = 4096;  // bytes of LDS a wave turns its output around in
+
+constexpr int lds_bytes(int kWB) {
+  const int tile = 64 * kWB;
+  const int ring = kStages * 2 * tile * kStageK, scales = kScaleRing * 2 * tile * 4;
+  return kWB == 4 ? ring + scales + kBiasRing * tile * 4 + 4 * kWaveStage : ring + scales + tile * 4;
+}
+
 template <int kWB, bool kWide>
 __global__ __launch_bounds__(kThreads) void fp8_gemm_kernel(const Problems P) {
+  constexpr bool kStream = kWB == 4;           // several tiles per workgroup, as one stream of stages
   constexpr int kTile = 64 * kWB;
   constexpr int kSlab = kTile * kStageK;       // bytes of one operand's stage
   constexpr int kStageBytes = 2 * kSlab;
   constexpr int kPieces = kTile / 64;          // 16-row loads per wave, stage and operand
+  constexpr int kLoads = 2 * kPieces;          // per wave and stage
   constexpr int kScaleLoads = kTile / 128;     // 64-row scale loads per wave and group (both operands)
   constexpr int kScaleBytes = 2 * kTile * 4;   // one group's scales: X rows, then W rows
   extern __shared__ __attribute__((aligned(16))) char smem[];
   char* scale_smem = smem + kStages * kStageBytes;
-  float* bias_smem = reinterpret_cast<float*>(scale_smem + 2 * kScaleBytes);
+  char* bias_smem = scale_smem + kScaleRing * kScaleBytes;
+  [[maybe_unused]] char* turn_smem = bias_smem + kBiasRing * kTile * 4;  // (kStream)
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = wave >> 1, wj = wave & 1;
   const int r = lane & 31, h = lane >> 5;
 
-  const int padded0 = (P.p[0].tasks + 7) & ~7;
-  const bool second = (int)blockIdx.x >= padded0;
-  const Problem& pr = P.p[second];
-  const int local = blockIdx.x - (second ? padded0 : 0);
-  if (local >= pr.tasks) return;  // padding
-  const Operand &X = pr.x, &W = pr.w;
-  const int M = X.rows, N = W.rows;
-
-  // Tasks are dealt to the 8 XCDs in contiguous ranges; consecutive tasks walk kGroupM token tiles x all
-  // feature tiles, so the workgroups of an XCD share operand rows in its L2.
-  const int tiles_m = (M + kTile - 1) / kTile, tiles_n = (N + kTile - 1) / kTile;
-  const int n_tiles = tiles_m * tiles_n;
-  const int q8 = pr.tasks / 8, r8 = pr.tasks % 8;
-  const int xcd = local % 8, within = local / 8;
-  const int task = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + within;
-  const int slice = task / n_tiles;
-  const int tile = task - slice * n_tiles;
-  const int group = tile / (kGroupM * tiles_n);
-  const int in_group = tile - group * (kGroupM * tiles_n);
-  const int group_rows = min(kGroupM, tiles_m - group * kGroupM);
-  const int m0 = (group * kGroupM + in_group % group_rows) * kTile;
-  const int n0 = (in_group / group_rows) * kTile;
-  const int first = slice * pr.steps_per_slice;  // a multiple of kGroupStages
-  const int n_steps = min(pr.steps_per_slice, pr.steps - first);
-
-  for (int i = threadIdx.x; i < kTile; i += kThreads) {  // read by the epilogue, many barriers from here
-    float v = 0.f;
-    if (pr.bias && n0 + i < N)
-      v = pr.bias_f32 ? ((const float*)pr.bias)[n0 + i] : bf16_to_f32(((const bf16_raw*)pr.bias)[n0 + i]);
-    bias_smem[i] = v;
+  Place at = place_of<kTile>(P, blockIdx.x, gridDim.x, 0);  // what is computed; every workgroup has a first task
+  if constexpr (!kStream) {
+    const Problem& pr = P.p[at.which];
+    for (int i = threadIdx.x; i < kTile; i += kThreads) {  // read by the epilogue, many barriers from here
+      float v = 0.f;
+      if (pr.bias && at.n0 + i < pr.w.rows)
+        v = pr.bias_f32 ? ((const float*)pr.bias)[at.n0 + i] : bf16_to_f32(((const bf16_raw*)pr.bias)[at.n0 + i]);
+      reinterpret_cast<float*>(bias_smem)[i] = v;
+    }
   }
 
-  // ---- staging: piece i of a slab = rows (kTile / 4) wave + 16 i .. +15, lane p -> row + p / 4, slot p % 4.
+  // ---- staging: the loads' own cursor, kStages stages ahead of the products and across tiles.
+  // Piece i of a slab = rows (kTile / 4) wave + 16 i .. +15, lane p -> row + p / 4, slot p % 4.
   // Rows past the end repeat the last one (never stored).
   // (All offsets fit 32 bits: a tile's rows span at most 256 * 2^22 bytes, a bound the host checks.)
-  const int x_rows = min(M - m0, kTile), w_rows = min(N - n0, kTile);
-  const unsigned k_bytes = (unsigned)n_steps * kStageK;
-  const auto x_src = bounded(X.q + int64_t(m0) * X.ld + int64_t(first) * kStageK, (unsigned)(x_rows - 1) * (unsigned)X.ld + k_bytes);
-  const auto w_src = bounded(W.q + int64_t(n0) * W.ld + int64_t(first) * kStageK, (unsigned)(w_rows - 1) * (unsigned)W.ld + k_bytes);
-  unsigned x_off[kPieces], w_off[kPieces];
+  // Scales: group g = blocks 4 g .. 4 g + 3 of the slice, a dword per row; 64 rows per load, all of one operand:
+  // waves 0, 1 fetch the scales of X's rows, waves 2, 3 those of W's.
+  __amdgpu_buffer_rsrc_t x_src, w_src, s_src;
+  unsigned x_off[kPieces], w_off[kPieces], s_off[kScaleLoads];
+  int c_round = 0, c_step = 0, c_steps = 0, c_groups = 0;
+  bool c_done = false;
+  auto aim = [&](const Place& to) {
+    const Operand &X = P.p[to.which].x, &W = P.p[to.which].w;
+    const int x_rows = min(X.rows - to.m0, kTile), w_rows = min(W.rows - to.n0, kTile);
+    const unsigned k_bytes = (unsigned)to.n_steps * kStageK;
+    x_src = bounded(X.q + int64_t(to.m0) * X.ld + int64_t(to.first) * kStageK, (unsigned)(x_rows - 1) * (unsigned)X.ld + k_bytes);
+    w_src = bounded(W.q + int64_t(to.n0) * W.ld + int64_t(to.first) * kStageK, (unsigned)(w_rows - 1) * (unsigned)W.ld + k_bytes);
 #pragma unroll
-  for (int i = 0; i < kPieces; ++i) {
-    const int row = (kTile / 4) * wave + 16 * i + (lane >> 2);
-    const unsigned chunk = (unsigned)(((lane & 3) ^ ((row >> 2) & 3)) * 16);
-    x_off[i] = (unsigned)min(row, x_rows - 1) * (unsigned)X.ld + chunk;
-    w_off[i] = (unsigned)min(row, w_rows - 1) * (unsigned)W.ld + chunk;
-  }
-  auto issue_one = [&](int t, int slot, int i) {  // i < 2 kPieces
-    const unsigned ko = (unsigned)min(t, n_steps - 1) * kStageK;  // past the end: the last stage again (never used)
+    for (int i = 0; i < kPieces; ++i) {
+      const int row = (kTile / 4) * wave + 16 * i + (lane >> 2);
+      const unsigned chunk = (unsigned)(((lane & 3) ^ ((row >> 2) & 3)) * 16);
+      x_off[i] = (unsigned)min(row, x_rows - 1) * (unsigned)X.ld + chunk;
+      w_off[i] = (unsigned)min(row, w_rows - 1) * (unsigned)W.ld + chunk;
+    }
+    const Operand& s_op = wave < 2 ? X : W;
+    const int s_row0 = wave < 2 ? to.m0 : to.n0, s_last = s_op.rows - 1;
+    const int s_lo = s_row0 >> s_op.shift, s_hi = min(s_row0 + kTile - 1, s_last) >> s_op.shift;
+    s_src = bounded(s_op.scale + int64_t(s_lo) * s_op.ld_scale + to.first / 2,
+                    (unsigned)(s_hi - s_lo) * (unsigned)s_op.ld_scale + 4u * (unsigned)((to.n_steps + kGroupStages - 1) / kGroupStages));
+#pragma unroll
+    for (int i = 0; i < kScaleLoads; ++i) {
+      const int row = ((wave & 1) * kScaleLoads + i) * 64 + lane;
+      s_off[i] = (unsigned)((min(s_row0 + row, s_last) >> s_op.shift) - s_lo) * (unsigned)s_op.ld_scale;
+    }
+    c_step = 0;
+    c_steps = to.n_steps;
+    if constexpr (kStream) {
+      // the tile's bias as it lies there, fp32 or pairs of bf16 (whole dwords: 4-byte aligned, a bound the host checks)
+      const Problem& pr = P.p[to.which];
+      if (pr.bias && (pr.bias_f32 || wave < 2)) {
+        const unsigned size = pr.bias_f32 ? 4u : 2u;
+        const auto b_src = bounded((const uint8_t*)pr.bias + (unsigned)to.n0 * size, ((unsigned)w_rows * size + 3u) & ~3u);
+        load_to_lds4(b_src, (unsigned)(wave * 64 + lane) * 4u, 0, bias_smem + (c_round & (kBiasRing - 1)) * kTile * 4 + wave * 256);
+      }
+    }
+  };
+  // Before the loads of an even stage: on to the next tile where this one ends (after the last, its last two stages
+  // again, never used), and the scales of a new group.
+  auto turn = [&]() {
+    if (c_step == c_steps) {
+      Place to;
+      to.which = -1;
+      if constexpr (kStream) {
+        if (!c_done) to = place_of<kTile>(P, blockIdx.x, gridDim.x, ++c_round);
+      }
+      if (to.which < 0) {
+        c_done = true;
+        c_step = c_steps - 2;
+      } else {
+        aim(to);
+      }
+    }
+    if ((c_step & (kGroupStages - 1)) == 0 && !c_done) {
+#pragma unroll
+      for (int i = 0; i < kScaleLoads; ++i)
+        load_to_lds4(s_src, s_off[i], 4u * (unsigned)(c_step / kGroupStages),
+                     scale_smem + (c_groups & (kScaleRing - 1)) * kScaleBytes + (wave * kScaleLoads + i) * 256);
+      ++c_groups;
+    }
+  };
+  auto issue_one = [&](int slot, int i) {  // i < kLoads
+    const unsigned ko = (unsigned)c_step * kStageK;
     char* dst = smem + slot * kStageBytes + ((kTile / 4) * wave + 16 * (i % kPieces)) * kStageK;
     if (i < kPieces) load_to_lds16(x_src, x_off[i], ko, dst);
     else load_to_lds16(w_src, w_off[i - kPieces], ko, dst + kSlab);
   };
-  // ---- scales: group g = blocks 4 g .. 4 g + 3, a dword per row; 64 rows per load, all of one operand.
-  const int n_groups = (n_steps + kGroupStages - 1) / kGroupStages;
-  const bool s_of_x = wave < 2;  // waves 0, 1 fetch the scales of X's rows, waves 2, 3 those of W's
-  const Operand& s_op = s_of_x ? X : W;
-  const int s_row0 = s_of_x ? m0 : n0, s_last = (s_of_x ? M : N) - 1;
-  const int s_lo = s_row0 >> s_op.shift, s_hi = min(s_row0 + kTile - 1, s_last) >> s_op.shift;
-  const auto s_src = bounded(s_op.scale + int64_t(s_lo) * s_op.ld_scale + first / 2,
-                             (unsigned)(s_hi - s_lo) * (unsigned)s_op.ld_scale + 4u * (unsigned)n_groups);
-  unsigned s_off[kScaleLoads];
-#pragma unroll
-  for (int i = 0; i < kScaleLoads; ++i) {
-    const int row = ((wave & 1) * kScaleLoads + i) * 64 + lane;
-    s_off[i] = (unsigned)((min(s_row0 + row, s_last) >> s_op.shift) - s_lo) * (unsigned)s_op.ld_scale;
-  }
-  auto issue_scales = [&](int g) {
-#pragma unroll
-    for (int i = 0; i < kScaleLoads; ++i)
-      load_to_lds4(s_src, s_off[i], 4u * (unsigned)min(g, n_groups - 1),
-                   scale_smem + (g & 1) * kScaleBytes + (wave * kScaleLoads + i) * 256);
-  };
 
   f32x16 acc[kWB][kWB];
-#pragma unroll
-  for (int a = 0; a < kWB; ++a)
-#pragma unroll
-    for (int b = 0; b < kWB; ++b)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[a][b][e] = 0.f;
 
   // ---- fragment addresses: lane (r, h) reads chunks h and 2 + h of row r of each 32-row block
   const unsigned smem_base = lds_addr(smem);
@@ -236,12 +302,19 @@ __global__ __launch_bounds__(kThreads) void fp8_gemm_kernel(const Problems P) {
     for (int b = 0; b < kWB; ++b)
       asm volatile("" : "+v"(xf[buf][b][0]), "+v"(xf[buf][b][1]), "+v"(wf[buf][b][0]), "+v"(wf[buf][b][1]));
   };
-  // scale bytes of block c (a pair of stages), read 0 .. 2 kWB - 1: X's and W's of each 32-row block in turn
+  // scale bytes of the next block (a pair of stages), read 0 .. 2 kWB - 1: X's and W's of each 32-row block in turn
   const unsigned scale_base = lds_addr(scale_smem);
   const unsigned xs_row = (unsigned)((32 * kWB * wi + r) * 4), ws_row = (unsigned)((kTile + 32 * kWB * wj + r) * 4);
   uint32_t xs[kWB], ws[kWB], xs_next[kWB], ws_next[kWB];
-  auto read_scale = [&](int c, int i) {
-    const unsigned at = scale_base + ((c >> 2) & 1) * kScaleBytes + (c & 3) + ((i & 1) ? ws_row : xs_row);
+  unsigned scale_at = scale_base;  // of the block that is read next
+  int block = 0, groups = 0;       // its place: block of the tile, group of the workgroup's stream
+  auto next_block = [&](bool tile_ends) {
+    block = tile_ends ? 0 : block + 1;
+    if ((block & 3) == 0) ++groups;
+    scale_at = scale_base + (groups & (kScaleRing - 1)) * kScaleBytes + (block & 3);
+  };
+  auto read_scale = [&](int i) {
+    const unsigned at = scale_at + ((i & 1) ? ws_row : xs_row);
     uint32_t& dst = (i & 1) ? ws_next[i >> 1] : xs_next[i >> 1];
     if ((i >> 1) == 0) asm volatile("ds_read_u8 %0, %1" : "=v"(dst) : "v"(at));
     if ((i >> 1) == 1) asm volatile("ds_read_u8 %0, %1 offset:128" : "=v"(dst) : "v"(at));
@@ -256,144 +329,263 @@ __global__ __launch_bounds__(kThreads) void fp8_gemm_kernel(const Problems P) {
       ws[b] = ws_next[b];
     }
   };
-  constexpr int kLoads = 2 * kPieces;  // per wave and stage
 
-  issue_scales(0);
+  aim(at);
 #pragma unroll
-  for (int t = 0; t < kStages; ++t)
+  for (int t = 0; t < kStages; ++t) {
+    if (t % 2 == 0) turn();
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) issue_one(t, t, i);
+    for (int i = 0; i < kLoads; ++i) issue_one(t, i);
+    ++c_step;
+  }
   if constexpr (kWB == 4) asm volatile("s_waitcnt vmcnt(24)" ::: "memory");
   else asm volatile("s_waitcnt vmcnt(12)" ::: "memory");
   __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-  for (int i = 0; i < 2 * kWB; ++i) read_scale(0, i);
+  for (int i = 0; i < 2 * kWB; ++i) read_scale(i);
 #pragma unroll
   for (int i = 0; i < 4 * kWB; ++i) frag(0, 0, i);
   await_frags(0);
   take_scales();
 
-  int slot = 0;  // of stage t
-  for (int t = 0; t < n_steps; t += 2) {  // n_steps is even; a pair of stages is one scale block
-    if ((t & (kGroupStages - 1)) == 0) issue_scales(t / kGroupStages + 1);
+  int slot = 0;   // of the stage in hand
+  int fresh = 0;  // stages since an epilogue left its stores in flight: see below
+  for (int round = 0;;) {
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      // Stage t + u + 1 has landed (two younger stages may be in flight; a scale load among them makes the
-      // count strict by that much); after the barrier everyone's part has, and nobody reads this slot any more.
-      if constexpr (kWB == 4) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
-      else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-      __builtin_amdgcn_sched_barrier(0);
-      const int next = (slot + 1) & (kStages - 1);
-      constexpr int kProducts = kWB * kWB;
-      int reads = 0, loads = 0, scales = 0;
-      [[maybe_unused]] bf16x8 xb[4], wb[kWide ? kWB : 1][4];
+    for (int a = 0; a < kWB; ++a)
 #pragma unroll
-      for (int i = 0; i < kProducts; ++i) {
-        const int a = i / kWB, b = i % kWB;
-        if constexpr (kWide) {
-          if (b == 0) {
+      for (int b = 0; b < kWB; ++b)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) xb[k] = widen8(xf[u][a][k >> 1][2 * (k & 1)], xf[u][a][k >> 1][2 * (k & 1) + 1], xs[a]);
-          }
-          if (a == 0) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) wb[b][k] = widen8(wf[u][b][k >> 1][2 * (k & 1)], wf[u][b][k >> 1][2 * (k & 1) + 1], ws[b]);
-          }
-#pragma unroll
-          for (int k = 0; k < 4; ++k) acc[a][b] = attn::mfma32(wb[b][k], xb[k], acc[a][b]);
-        } else {
-          acc[a][b] = mfma_scaled(join(wf[u][b][0], wf[u][b][1]), join(xf[u][a][0], xf[u][a][1]), acc[a][b], ws[b], xs[a]);
-        }
-#pragma unroll
-        for (; reads < (i + 1) * 4 * kWB / kProducts; ++reads) frag(u ^ 1, next, reads);
-        if (u == 1) {
-#pragma unroll
-          for (; scales < (i + 1) * 2 * kWB / kProducts; ++scales) read_scale(t / 2 + 1, scales);
-        }
-#pragma unroll
-        for (; loads < (i + 1) * kLoads / kProducts; ++loads) issue_one(t + u + kStages, slot, loads);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      await_frags(u ^ 1);
-      __builtin_amdgcn_sched_barrier(0);
-      slot = next;
-    }
-    take_scales();
-  }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the tail's unused loads have left LDS alone
-  __syncthreads();                                  // and nobody reads the ring any more: it stages the output
+        for (int e = 0; e < 16; ++e) acc[a][b][e] = 0.f;
 
-  // ---- epilogue: register e of acc[a][b]: token m0 + 32 kWB wi + 32 a + r, feature n0 + 32 kWB wj + 32 b +
-  // 8 (e / 4) + 4 h + (e & 3). Through LDS, so that rows leave in whole lines: staged row = token, its 16-byte
-  // chunks XOR-permuted with the token, so the lanes of a write (32 tokens, one feature offset) and of a read
-  // (one token) both spread over the banks. Written in `passes` passes of the a-blocks that fit the ring.
-  auto store_tile = [&](auto out_f32, auto passes) {
-    using Out = std::conditional_t<decltype(out_f32)::value, float, bf16_raw>;
-    constexpr int kRowBytes = kTile * (int)sizeof(Out), kVec = 16 / (int)sizeof(Out);
-    constexpr int kPasses = decltype(passes)::value, kBlocks = kWB / kPasses, kRows = 64 * kBlocks;
-    constexpr int kChunks = kRowBytes / 16;
-    Out* out = (Out*)pr.out + int64_t(slice) * M * N;
+    for (int t = 0; t < at.n_steps; t += 2) {  // n_steps is even; a pair of stages is one scale block
+      next_block(t + 2 == at.n_steps);
 #pragma unroll
-    for (int pass = 0; pass < kPasses; ++pass) {
-#pragma unroll
-      for (int ai = 0; ai < kBlocks; ++ai)
-#pragma unroll
-        for (int b = 0; b < kWB; ++b) {
-          f32x16 v = acc[pass * kBlocks + ai][b];
-          asm volatile("" : "+v"(v));  // one block at a time leaves the accumulator file
-          const int row = 32 * (kBlocks * wi + ai) + r;
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            const int col = 32 * (kWB * wj + b) + 8 * g + 4 * h;
-            const f32x4 bv = *reinterpret_cast<const f32x4*>(bias_smem + col);
-            const int at = row * kRowBytes + (((col / kVec) ^ (r & (kChunks - 1))) * 16) + (col % kVec) * (int)sizeof(Out);
-            if constexpr (sizeof(Out) == 2)
-              *reinterpret_cast<u32x2*>(smem + at) = u32x2{pack_bf16x2(v[4 * g] + bv[0], v[4 * g + 1] + bv[1]),
-                                                          pack_bf16x2(v[4 * g + 2] + bv[2], v[4 * g + 3] + bv[3])};
-            else
-              *reinterpret_cast<f32x4*>(smem + at) = f32x4{v[4 * g] + bv[0], v[4 * g + 1] + bv[1], v[4 * g + 2] + bv[2], v[4 * g + 3] + bv[3]};
-          }
+      for (int u = 0; u < 2; ++u) {
+        // Stage t + u + 1 has landed: two younger stages may be in flight (anything else among them makes the count
+        // strict by that much), and in the first three stages after an epilogue its stores too, which lie between
+        // that stage and the youngest. After the barrier everyone's part has, and nobody reads this slot any more.
+        if constexpr (kWB == 4) {
+          // (the branch is inside the block: around a branch of its own the compiler would sink products)
+          asm volatile("s_cmp_gt_i32 %0, 0\n\ts_cbranch_scc1 .Lfresh%=\n\ts_waitcnt vmcnt(16)\n.Lfresh%=:\n\ts_waitcnt vmcnt(48)"
+                       ::"s"(fresh)
+                       : "memory", "scc");
+          fresh = max(fresh - 1, 0);
+        } else {
+          asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
         }
-      __syncthreads();
-      // staged row q is token 32 kWB (q / 32 / kBlocks) + 32 (pass kBlocks + q / 32 % kBlocks) + q % 32 of the tile
-      auto token = [&](int q) {
-        const int blk = q >> 5;
-        return m0 + 32 * (kWB * (blk / kBlocks) + pass * kBlocks + blk % kBlocks) + (q & 31);
-      };
-      if (pr.vec) {
-        const int ch = threadIdx.x % kChunks, n = n0 + ch * kVec;
-        if (n < N) {  // (rows are whole chunks here)
-#pragma unroll 4
-          for (int q = threadIdx.x / kChunks; q < kRows; q += kThreads / kChunks) {
-            const int m = token(q);
-            const u32x4 w = *reinterpret_cast<const u32x4*>(smem + q * kRowBytes + ((ch ^ (q & 31 & (kChunks - 1))) * 16));
-            if (m < M) *reinterpret_cast<u32x4*>(out + int64_t(m) * N + n) = w;
+        __builtin_amdgcn_s_barrier();
+        if (u == 0) turn();
+        __builtin_amdgcn_sched_barrier(0);
+        const int next = (slot + 1) & (kStages - 1);
+        constexpr int kProducts = kWB * kWB;
+        int reads = 0, loads = 0, scales = 0;
+        [[maybe_unused]] bf16x8 xb[4], wb[kWide ? kWB : 1][4];
+#pragma unroll
+        for (int i = 0; i < kProducts; ++i) {
+          const int a = i / kWB, b = i % kWB;
+          if constexpr (kWide) {
+            if (b == 0) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) xb[k] = widen8(xf[u][a][k >> 1][2 * (k & 1)], xf[u][a][k >> 1][2 * (k & 1) + 1], xs[a]);
+            }
+            if (a == 0) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) wb[b][k] = widen8(wf[u][b][k >> 1][2 * (k & 1)], wf[u][b][k >> 1][2 * (k & 1) + 1], ws[b]);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[a][b] = attn::mfma32(wb[b][k], xb[k], acc[a][b]);
+          } else {
+            acc[a][b] = mfma_scaled(join(wf[u][b][0], wf[u][b][1]), join(xf[u][a][0], xf[u][a][1]), acc[a][b], ws[b], xs[a]);
           }
-        }
-      } else {  // rows at any alignment: an element per lane, neighbours in neighbouring lanes
-        const int col = threadIdx.x % kTile, n = n0 + col;
-        if (n < N) {
-#pragma unroll 4
-          for (int q = threadIdx.x / kTile; q < kRows; q += kThreads / kTile) {
-            const int m = token(q);
-            const Out w = *reinterpret_cast<const Out*>(smem + q * kRowBytes + (((col / kVec) ^ (q & 31 & (kChunks - 1))) * 16) +
-                                                        (col % kVec) * (int)sizeof(Out));
-            if (m < M) out[int64_t(m) * N + n] = w;
+#pragma unroll
+          for (; reads < (i + 1) * 4 * kWB / kProducts; ++reads) frag(u ^ 1, next, reads);
+          if (u == 1) {
+#pragma unroll
+            for (; scales < (i + 1) * 2 * kWB / kProducts; ++scales) read_scale(scales);
           }
+#pragma unroll
+          for (; loads < (i + 1) * kLoads / kProducts; ++loads) issue_one(slot, loads);
+          __builtin_amdgcn_sched_barrier(0);
         }
+        ++c_step;
+        await_frags(u ^ 1);
+        __builtin_amdgcn_sched_barrier(0);
+        slot = next;
       }
-      if (pass + 1 < kPasses) __syncthreads();
+      take_scales();
     }
-  };
-  if constexpr (kWide) {
-    store_tile(std::true_type{}, std::integral_constant<int, 1>{});
-  } else if (pr.out_f32) {
-    store_tile(std::true_type{}, std::integral_constant<int, kWB / 2>{});
-  } else {
-    store_tile(std::false_type{}, std::integral_constant<int, 1>{});
+
+    // ---- epilogue: register e of acc[a][b]: token m0 + 32 kWB wi + 32 a + r, feature n0 + 32 kWB wj + 32 b +
+    // 8 (e / 4) + 4 h + (e & 3). Through LDS, so that rows leave in whole lines: staged row = token, its 16-byte
+    // chunks XOR-permuted with the token, so the lanes of a write (32 tokens, one feature offset) and of a read
+    // (whole tokens) both spread over the banks.
+    const Problem& pr = P.p[at.which];
+    const int M = pr.x.rows, N = pr.w.rows;
+    const int m0 = at.m0, n0 = at.n0;
+    const int64_t slice0 = int64_t(at.slice) * M * N;
+    if constexpr (kStream) {
+      // The next tile's loads are on their way and its first fragments in registers: a wave turns its quarter around
+      // in 4 KiB of its own, 32 tokens x 128 bytes at a time, meets nobody, and goes on without waiting for its
+      // stores. LDS by inline assembly (in order within a wave): the compiler would wait for the loads in flight.
+#pragma unroll
+      for (int a = 0; a < kWB; ++a)
+#pragma unroll
+        for (int b = 0; b < kWB; ++b) asm volatile("" : "+a"(acc[a][b]));
+      int el = lane;
+      asm volatile("" : "+v"(el));  // (addresses are formed here, not held through the products)
+      const int er = el & 31, eh = el >> 5;
+      const int vec = __builtin_amdgcn_readfirstlane(pr.vec), bias_f32 = __builtin_amdgcn_readfirstlane(pr.bias_f32);
+      const int has_bias = __builtin_amdgcn_readfirstlane(pr.bias != nullptr);  // (held: not fetched after every store)
+      auto store_quarter = [&](auto out_f32) {
+        using Out = std::conditional_t<decltype(out_f32)::value, float, bf16_raw>;
+        constexpr int kSize = (int)sizeof(Out), kVec = 16 / kSize, kB = 4 / kSize;  // kB: feature blocks turned together
+        Out* out = (Out*)pr.out + slice0 + int64_t(m0) * N;
+        const auto dst = __builtin_amdgcn_make_buffer_rsrc((void*)out, 0, (int)((unsigned)min(M - m0, kTile) * (unsigned)N * kSize), 0x00027000);
+        const unsigned turn_base = lds_addr(turn_smem) + wave * kWaveStage;
+        const unsigned bias_base = lds_addr(bias_smem) + (round & (kBiasRing - 1)) * kTile * 4;
+#pragma unroll
+        for (int b0 = 0; b0 < kWB; b0 += kB) {
+          f32x4 bv[kB][4];
+#pragma unroll
+          for (int i = 0; i < 4 * kB; ++i) bv[i / 4][i % 4] = f32x4{0.f, 0.f, 0.f, 0.f};
+          const unsigned b_col = (unsigned)(32 * (kWB * wj + b0) + 4 * eh);
+          if (has_bias && bias_f32) {
+#pragma unroll
+            for (int i = 0; i < 4 * kB; ++i) asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(bv[i / 4][i % 4]) : "v"(bias_base + b_col * 4), "i"(32 * i));
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+            for (int i = 0; i < 4 * kB; ++i) asm volatile("" : "+v"(bv[i / 4][i % 4]));
+          } else if (has_bias) {
+            u32x2 w[4 * kB];
+#pragma unroll
+            for (int i = 0; i < 4 * kB; ++i) asm volatile("ds_read_b64 %0, %1 offset:%2" : "=v"(w[i]) : "v"(bias_base + b_col * 2), "i"(16 * i));
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+            for (int i = 0; i < 4 * kB; ++i) {
+              asm volatile("" : "+v"(w[i]));
+              bv[i / 4][i % 4] = f32x4{__uint_as_float(w[i][0] << 16), __uint_as_float(w[i][0] & 0xffff0000u),
+                                       __uint_as_float(w[i][1] << 16), __uint_as_float(w[i][1] & 0xffff0000u)};
+            }
+          }
+          const int col = n0 + 32 * (kWB * wj + b0) + (el & 7) * kVec;
+          const unsigned at0 = col < N ? ((unsigned)(32 * kWB * wi + (el >> 3)) * (unsigned)N + (unsigned)col) * kSize : 0x80000000u;
+          using Piece = std::conditional_t<kSize == 2, u32x2, f32x4>;  // four features of a token
+          Piece piece[kB][4];
+          auto round_up = [&](int a) {  // one block at a time leaves the accumulator file
+#pragma unroll
+            for (int b = 0; b < kB; ++b) {
+              f32x16 v = acc[a][b0 + b];
+              asm volatile("" : "+v"(v));
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {
+                const f32x4 y = f32x4{v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]} + bv[b][g];
+                if constexpr (kSize == 2) piece[b][g] = u32x2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+                else piece[b][g] = y;
+              }
+            }
+          };
+          round_up(0);
+#pragma unroll
+          for (int a = 0; a < kWB; ++a) {
+#pragma unroll
+            for (int b = 0; b < kB; ++b)
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {
+                const unsigned chunk = (unsigned)(32 * b + 8 * g + 4 * eh) / kVec;
+                const unsigned to = turn_base + er * 128 + ((chunk ^ (er & 7)) << 4) + (kSize == 2 ? 8 * eh : 0);
+                if constexpr (kSize == 2) asm volatile("ds_write_b64 %0, %1" ::"v"(to), "v"(piece[b][g]) : "memory");
+                else asm volatile("ds_write_b128 %0, %1" ::"v"(to), "v"(piece[b][g]) : "memory");
+              }
+            u32x4 w[4];
+            const unsigned from = turn_base + (el >> 3) * 128 + (((el & 7) ^ (el >> 3)) << 4);
+            w[0] = chunk_read<0>(from);
+            w[1] = chunk_read<1024>(from);
+            w[2] = chunk_read<2048>(from);
+            w[3] = chunk_read<3072>(from);
+            if (a + 1 < kWB) round_up(a + 1);  // while they come
+            asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3])::"memory");
+            // out of range (rows past M, columns past N): dropped, but issued and counted
+            if (vec) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                __builtin_amdgcn_raw_buffer_store_b128(w[i], dst, (int)(at0 + (unsigned)((32 * a + 8 * i) * N) * kSize), 0, 0);
+            } else {  // rows at any alignment: one element at a time
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) {
+                  const unsigned to = col + e < N ? at0 + (unsigned)((32 * a + 8 * i) * N + e) * kSize : 0x80000000u;
+                  if constexpr (kSize == 4) __builtin_amdgcn_raw_buffer_store_b32(w[i][e], dst, (int)to, 0, 0);
+                  else __builtin_amdgcn_raw_buffer_store_b16((unsigned short)(w[i][e / 2] >> (16 * (e & 1))), dst, (int)to, 0, 0);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+      };
+      // (at least 32 stores of a wave: the count of the three stages that follow)
+      if (pr.out_f32) store_quarter(std::true_type{});
+      else store_quarter(std::false_type{});
+      fresh = 3;
+      at = place_of<kTile>(P, blockIdx.x, gridDim.x, ++round);
+      if (at.which < 0) break;
+    } else {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the tail's unused loads have left LDS alone
+      __syncthreads();                                  // and nobody reads the ring any more: it stages the output
+      auto store_tile = [&](auto out_f32) {
+        using Out = std::conditional_t<decltype(out_f32)::value, float, bf16_raw>;
+        constexpr int kRowBytes = kTile * (int)sizeof(Out), kVec = 16 / (int)sizeof(Out);
+        constexpr int kChunks = kRowBytes / 16;
+        Out* out = (Out*)pr.out + slice0;
+#pragma unroll
+        for (int a = 0; a < kWB; ++a)
+#pragma unroll
+          for (int b = 0; b < kWB; ++b) {
+            f32x16 v = acc[a][b];
+            asm volatile("" : "+v"(v));  // one block at a time leaves the accumulator file
+            const int row = 32 * (kWB * wi + a) + r;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const int col = 32 * (kWB * wj + b) + 8 * g + 4 * h;
+              const f32x4 bv = *reinterpret_cast<const f32x4*>(bias_smem + col * 4);
+              const int to = row * kRowBytes + (((col / kVec) ^ (r & (kChunks - 1))) * 16) + (col % kVec) * (int)sizeof(Out);
+              if constexpr (sizeof(Out) == 2)
+                *reinterpret_cast<u32x2*>(smem + to) = u32x2{pack_bf16x2(v[4 * g] + bv[0], v[4 * g + 1] + bv[1]),
+                                                            pack_bf16x2(v[4 * g + 2] + bv[2], v[4 * g + 3] + bv[3])};
+              else
+                *reinterpret_cast<f32x4*>(smem + to) = f32x4{v[4 * g] + bv[0], v[4 * g + 1] + bv[1], v[4 * g + 2] + bv[2], v[4 * g + 3] + bv[3]};
+            }
+          }
+        __syncthreads();
+        if (pr.vec) {
+          const int ch = threadIdx.x % kChunks, n = n0 + ch * kVec;
+          if (n < N) {  // (rows are whole chunks here)
+#pragma unroll 4
+            for (int q = threadIdx.x / kChunks; q < kTile; q += kThreads / kChunks) {
+              const u32x4 w = *reinterpret_cast<const u32x4*>(smem + q * kRowBytes + ((ch ^ (q & 31 & (kChunks - 1))) * 16));
+              if (m0 + q < M) *reinterpret_cast<u32x4*>(out + int64_t(m0 + q) * N + n) = w;
+            }
+          }
+        } else {  // rows at any alignment: an element per lane, neighbours in neighbouring lanes
+          const int col = threadIdx.x % kTile, n = n0 + col;
+          if (n < N) {
+#pragma unroll 4
+            for (int q = threadIdx.x / kTile; q < kTile; q += kThreads / kTile) {
+              const Out w = *reinterpret_cast<const Out*>(smem + q * kRowBytes + (((col / kVec) ^ (q & 31 & (kChunks - 1))) * 16) +
+                                                          (col % kVec) * (int)sizeof(Out));
+              if (m0 + q < M) out[int64_t(m0 + q) * N + n] = w;
+            }
+          }
+        }
+      };
+      if (kWide || pr.out_f32) store_tile(std::true_type{});
+      else if constexpr (!kWide) store_tile(std::false_type{});
+      break;
+    }
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (kStream) no load to LDS outlives the workgroup
 }
 
 // out = (out +) bias + sum over `slices` of partial [slices][total], in a fixed order. Up to three such sums in
@@ -465,69 +657,124 @@ __global__ __launch_bounds__(kThreads) void fold_kernel(const Folds folds) {
 
 template <int kWB, bool kWide>
 void launch(const Problems& P, hipStream_t stream) {
-  constexpr int kTile = 64 * kWB;
-  constexpr int kLds = kStages * 2 * kTile * kStageK + 2 * 2 * kTile * 4 + kTile * 4;
+  constexpr int kLds = lds_bytes(kWB);
   (void)hipFuncSetAttribute((const void*)fp8_gemm_kernel<kWB, kWide>, hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
-  const unsigned blocks = (unsigned)(((P.p[0].tasks + 7) & ~7) + P.p[1].tasks);
+  const int tasks = P.p[0].tasks + P.p[1].tasks;
+  const unsigned blocks = (unsigned)(kWB == 4 ? std::min(tasks, kSlots) : tasks);
   hipLaunchKernelGGL((fp8_gemm_kernel<kWB, kWide>), dim3(blocks), dim3(kThreads), kLds, stream, P);
 }
 
 }  // namespace
 
-// Which tile, and how many slices of the contraction: the smallest estimated time. The estimate is rounds of
-// workgroups over the chip's slots, in microseconds fitted to measurements of 12 shapes from 16 x 3840 x 1280 to
-// 8192 x 22016 x 4096 (most within 10 %). A stage of a 256 tile takes 0.72 with every compute unit busy (0.47
-// alone); of a 128 tile 0.20 alone, 0.29 with one workgroup per compute unit, 0.60 with two. What else a
-// workgroup costs (first loads, stores) is 10 and 3.3. So 8192 x 1280 x 5120 takes the 256 tile (160 of them: 65
-// against 77), 2048^3 the 128 tile (13 against 28). A slice's partial sums are written and read again at some
-// 4.5 TB/s and folded by a launch of 3: 1024 x 1024 x 8192 gains by four slices (33 -> 23), 2048^3 loses by two
-// (13 -> 31). The widened products have the 128 tile only, at 1.5 times its stage.
-static float plan_time(int tile, int64_t tasks, int steps, bool wide) {
-  const int64_t slots = tile == 256 ? 256 : 512;
-  auto round = [&](int64_t n) {
-    const float load = n / 256.f;
-    if (tile == 256) return 10.f + steps * (0.47f + 0.25f * load);
+// Which tile, and how many slices of the contraction: the smallest estimated time, in microseconds fitted to
+// measurements of 14 shapes from 16 x 3840 x 1280 to 8192 x 22016 x 4096 (most within 10 %).
+// 256 tile: workgroups stream through their tasks, dealt as place_of does; a stage takes 0.75 with every compute
+// unit busy (0.47 alone), a tile 3 more (its epilogue), the launch 10 (first loads, last stores).
+// 128 tile: rounds of workgroups over two slots a compute unit; a stage takes 0.20 alone, 0.29 with one workgroup
+// per compute unit, 0.60 with two, a workgroup 3.3 more. The widened products have this tile only, at 1.5 times
+// its stage.
+// So 8192 x 1280 x 5120 takes the 256 tile (160 of them: 63 against 77), 2048^3 the 128 tile (13 against 28), and
+// the two gradients of 8192 x 1280 -> 5120 together the 256 tile (260 of two lengths: 128 against 162).
+// A slice's partial sums are written and read again at some 4.5 TB/s and folded by a launch of 3: 1024 x 1024 x
+// 8192 gains by four slices (33 -> 23), 2048^3 loses by two (13 -> 31).
+struct Work {
+  int64_t tasks;
+  int steps;
+};
+
+static float time_256(const Work* work, int n) {  // the longer tasks first
+  const int64_t first = work[0].tasks, total = first + (n > 1 ? work[1].tasks : 0);
+  const float stage = 0.47f + 0.28f * (total < kSlots ? total / float(kSlots) : 1.f);
+  auto task = [&](int64_t i) { return i >= total ? 0.f : 3.f + stage * work[i >= first].steps; };
+  const int64_t rounds = ceil_div(total, kSlots);
+  if (n == 1) return 10.f + rounds * task(0);
+  if (rounds > 32) return 10.f + (first * task(0) + (total - first) * task(total - 1)) / kSlots + task(total - 1);
+  float most = 0.f;
+  for (int w = 0; w < kSlots; w += 15) {  // (0 and 255 among them)
+    float t = 0.f;
+    for (int64_t r = 0; r < rounds; ++r) t += task(r * kSlots + ((r & 1) ? kSlots - 1 - w : w));
+    most = std::max(most, t);
+  }
+  return 10.f + most;
+}
+
+static float time_128(const Work* work, int n, bool wide) {
+  const int64_t slots = 2 * kSlots;
+  auto task = [&](int64_t tasks, int steps) {  // of so many at once
+    const float load = std::min(tasks, slots) / float(kSlots);
     const float stage = load <= 1.f ? 0.20f + 0.09f * load : 0.29f + 0.31f * (load - 1.f);
     return 3.3f + steps * stage * (wide ? 1.5f : 1.f);
   };
-  const int64_t full = tasks / slots, rest = tasks % slots;
-  return (tile == 256 ? 4.f : 1.4f) + full * round(slots) + (rest ? round(rest) : 0.f);
+  if (n == 1) {
+    const int64_t full = work[0].tasks / slots, rest = work[0].tasks % slots;
+    return 1.4f + full * task(slots, work[0].steps) + (rest ? task(rest, work[0].steps) : 0.f);
+  }
+  const int64_t total = work[0].tasks + work[1].tasks;
+  const float a = task(total, work[0].steps), b = task(total, work[1].steps);
+  if (total <= slots) return 1.4f + std::max(a, b);
+  return 1.4f + (work[0].tasks * a + work[1].tasks * b) / slots + 0.5f * std::max(a, b);
 }
 
-static Fp8GemmPlan plan_for_tile(int tile, int M, int N, int K, bool wide, float* time) {
-  const int steps = K / kStageK, groups = (steps + kGroupStages - 1) / kGroupStages;
-  const int64_t tiles = ceil_div(M, tile) * ceil_div(N, tile);
-  Fp8GemmPlan best{tile, 1, groups * kGroupStages};
-  *time = plan_time(tile, tiles, steps, wide);
-  for (int slices = 2; slices <= groups && slices <= 16; ++slices) {
-    const int per = (groups + slices - 1) / slices;
-    const int real = (groups + per - 1) / per;  // slices that have any work
-    if (real != slices) continue;
-    const float t = plan_time(tile, tiles * slices, per * kGroupStages, wide) + 3.f + float(M) * N * (8.f * slices + 2.f) / 4.5e6f;
-    if (t < *time) {
-      *time = t;
-      best = Fp8GemmPlan{tile, slices, per * kGroupStages};
+// Up to two products that share a launch: one tile for both, each cut or not.
+struct Choice {
+  Fp8GemmPlan plan[2];
+  float time;
+};
+
+static Work work_of(const Fp8GemmPlan& plan, const Fp8GemmProblem& p) {
+  return Work{ceil_div(p.x.rows, plan.tile) * ceil_div(p.w.rows, plan.tile) * plan.slices, std::min(plan.steps_per_slice, p.K / kStageK)};
+}
+static float fold_time(const Fp8GemmPlan& plan, const Fp8GemmProblem& p) {
+  return plan.slices == 1 ? 0.f : 3.f + float(p.x.rows) * p.w.rows * (8.f * plan.slices + 2.f) / 4.5e6f;
+}
+
+static float time_of(const Fp8GemmPlan* plans, const Fp8GemmProblem* problems, int n) {
+  Work work[2] = {};
+  float t = 0.f;
+  for (int i = 0; i < n; ++i) {
+    work[i] = work_of(plans[i], problems[i]);
+    t += fold_time(plans[i], problems[i]);
+  }
+  if (n == 2 && work[1].steps > work[0].steps) std::swap(work[0], work[1]);
+  return t + (plans[0].tile == 256 ? time_256(work, n) : time_128(work, n, problems[0].out_dtype == kF32));
+}
+
+static Choice choose(int tile, const Fp8GemmProblem* problems, int n) {
+  Choice best = {};
+  Fp8GemmPlan whole[2], cut[2];
+  for (int i = 0; i < n; ++i) {
+    const int groups = (problems[i].K / kStageK + kGroupStages - 1) / kGroupStages;
+    whole[i] = cut[i] = Fp8GemmPlan{tile, 1, groups * kGroupStages};
+    float least = time_of(&whole[i], &problems[i], 1);
+    for (int slices = 2; slices <= groups && slices <= 16; ++slices) {
+      const int per = (groups + slices - 1) / slices;
+      if ((groups + per - 1) / per != slices) continue;  // (a slice without work)
+      const Fp8GemmPlan plan{tile, slices, per * kGroupStages};
+      const float t = time_of(&plan, &problems[i], 1);
+      if (t < least) least = t, cut[i] = plan;
     }
+  }
+  for (int k = 0; k < (1 << n); ++k) {
+    Choice c = {};
+    for (int i = 0; i < n; ++i) c.plan[i] = (k >> i) & 1 ? cut[i] : whole[i];
+    c.time = time_of(c.plan, problems, n);
+    if (k == 0 || c.time < best.time) best = c;
   }
   return best;
 }
 
-// Products that run together take the tile that is best for their sum, so that they share a launch.
 void fp8_gemm_plan(Fp8GemmProblem* problems, int n) {
-  Fp8GemmPlan plans[2][2];
-  float sum[2] = {0.f, 0.f};
-  bool wide = false;
+  bool small = false;  // no 256 tile: widened products, or what its epilogue's 32-bit offsets and bias loads do not reach
   for (int i = 0; i < n; ++i) {
-    Fp8GemmProblem& p = problems[i];
-    wide |= p.out_dtype == kF32;
-    for (int k = 0; k < 2; ++k) {
-      float t;
-      plans[k][i] = plan_for_tile(k ? 256 : 128, p.x.rows, p.w.rows, p.K, p.out_dtype == kF32, &t);
-      sum[k] += t;
-    }
+    const Fp8GemmProblem& p = problems[i];
+    small |= p.out_dtype == kF32 || p.w.rows > (1 << 20) || reinterpret_cast<uintptr_t>(p.bias) % 4 != 0;
   }
-  const int k = !wide && sum[1] < sum[0];
-  for (int i = 0; i < n; ++i) problems[i].plan = plans[k][i];
+  Choice best = choose(128, problems, n);
+  if (!small) {
+    const Choice big = choose(256, problems, n);
+    if (big.time < best.time) best = big;
+  }
+  for (int i = 0; i < n; ++i) problems[i].plan = best.plan[i];
 }
 
 void fp8_gemm(const Fp8GemmProblem* problems, int n, const Fp8ColumnSums* sums, hipStream_t stream) {

@@ -111,6 +111,24 @@ def test_product(m, n, k, dtype, tiles):
         check_product(b, a, None, dtype, ops.fp8_matmul(b, a, None, dtype))  # tiles on the left
 
 
+@pytest.mark.parametrize("m,n,k", [(8192, 5120, 1280), (8100, 5001, 1300), (16500, 2600, 1400), (2000, 2048, 65536), (2000, 2001, 65536)])
+@pytest.mark.parametrize("bias", [None, torch.bfloat16, torch.float32])
+def test_product_of_many_tiles(m, n, k, bias):
+    """Sizes at which a workgroup goes through several tiles, and through slices of a long contraction."""
+    a, b = ops.quantize_fp8(rand(m, k, seed=1)), ops.quantize_fp8(rand(n, k, seed=2))
+    c = None if bias is None else rand(n, 1, seed=3)[:, 0].to(bias)
+    y = ops.fp8_matmul(a, b, c, torch.bfloat16)
+    check_product(a, b, c, torch.bfloat16, y)
+    for _ in range(3):
+        assert torch.equal(y, ops.fp8_matmul(a, b, c, torch.bfloat16))
+
+
+def test_bias_at_any_alignment():
+    a, b = ops.quantize_fp8(rand(8192, 1300, seed=1)), ops.quantize_fp8(rand(5001, 1300, seed=2))
+    c = rand(5003, 1, seed=3)[:, 0].bfloat16()[1:5002]
+    check_product(a, b, c, torch.bfloat16, ops.fp8_matmul(a, b, c, torch.bfloat16))
+
+
 def test_product_of_non_finite_values():
     x, w = rand(200, 300, seed=1), rand(140, 300, seed=2)
     x[3, 200], x[150, 7], w[9, 299] = math.inf, math.nan, -math.inf
@@ -151,7 +169,7 @@ def check_layer(x, w, b, dy, y, dx, dw, db):
             assert ((db.double() - want).abs() <= step * want.abs() + (dy.shape[0] / 128 + 16) * 2.0 ** -24 * size).all()
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (7, 40, 24), (200, 300, 129), (1000, 513, 257), (3000, 512, 1000)])
+@pytest.mark.parametrize("m,n,k", [(1, 1, 1), (7, 40, 24), (200, 300, 129), (1000, 513, 257), (3000, 512, 1000), (4096, 2560, 1280), (8200, 1203, 5127)])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_layer(m, n, k, dtype):
     x, w, b, dy = layer_case(m, n, k, dtype)
