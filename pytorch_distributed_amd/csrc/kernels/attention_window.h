@@ -87,6 +87,21 @@ struct TileAddr {
   }
 };
 
+// The same addresses out of three registers: steps, column blocks and halves only flip bits inside a row (tiles
+// start at multiples of a row), at an instruction per read.
+template <int D>
+struct TileAddrSmall {
+  unsigned row0, tr0, tr1;
+  __device__ __forceinline__ void init(unsigned base, int lane) {
+    TileAddr<D> at;
+    at.init(base, lane);
+    row0 = at.row[0], tr0 = at.tr[0][0], tr1 = at.tr[0][1];
+  }
+  __device__ __forceinline__ unsigned row(int ks) const { return row0 ^ (unsigned)(32 * ks); }
+  __device__ __forceinline__ unsigned tr(int db, int half) const { return (half ? tr1 : tr0) ^ (unsigned)(64 * db); }
+  __device__ __forceinline__ void move(int by) { row0 += by, tr0 += by, tr1 += by; }
+};
+
 // Moves 64-row tiles of [rows][D] bf16 (row pitch in bytes) into LDS, swizzled as tile_off: lane p of a wave's
 // load i lands on row 16 wave + i kRows + p / kChunks, slot p % kChunks, and fetches the chunk that belongs there.
 template <int D>
@@ -158,15 +173,15 @@ __device__ __forceinline__ bool visible(const Shape& s, int q, int key) {
   return key <= q && (q - key < s.window || key < s.sinks);
 }
 
-// Score accumulators [2 key halves][16] of a tile start from minus infinity where the query (on the lane) does not
-// see the key: the products leave it there, so the maximum ignores it and its probability is zero.
-__device__ __forceinline__ void start_masked(const Shape& s, int q_row, int q0, int key0, int h, f32x16 (&acc)[2]) {
-  if (!tile_masked(s, key0, q0)) return;  // wave-uniform
+// Score accumulators of the 32 keys from `key0` on start from minus infinity where the query (on the lane) does
+// not see the key: the products leave it there, so the maximum ignores it and its probability is zero.
+__device__ __forceinline__ void start_masked(const Shape& s, int q_row, int key0, int h, f32x16& acc) {
+  __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-  for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (!visible(s, q_row, key0 + kb * 32 + acc_row(i, h))) acc[kb][i] = -INFINITY;
+  for (int i = 0; i < 16; ++i) {
+    if (!visible(s, q_row, key0 + acc_row(i, h))) acc[i] = -INFINITY;
+    __builtin_amdgcn_sched_barrier(0);  // (few registers: one comparison at a time)
+  }
 }
 
 }  // namespace window

@@ -125,7 +125,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) s_acc[kb][i] = 0.f;
-      start_masked(s, q_row, q0, key0, h, s_acc);
+      if (tile_masked(s, key0, q0)) {  // wave-uniform
+        start_masked(s, q_row, key0, h, s_acc[0]);
+        start_masked(s, q_row, key0 + 32, h, s_acc[1]);
+      }
       static_for<0, kN>([&](auto n) {
         constexpr int kb = n % 2, ks = n / 2;
         wait_for<(kN - 1 - n < kAhead - 1 ? kN - 1 - n : kAhead - 1)>(kf[n % kAhead]);
@@ -232,10 +235,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
 // ============================================================================ dQ
 // S^T = K Q^T - lse / c, P^T = exp2(c S^T), dP^T = V dO^T - delta, dS^T = P^T dP^T, dQ^T += K^T dS^T: the
 // row constants are the accumulators' initial values. Also
-// delta = rowsum(dO O) for the dK / dV kernels. A tile is two 32-key halves; the second half's chains are issued
-// under the first one's exponentials, the first half's dQ products under the second one's.
+// delta = rowsum(dO O) for the dK / dV kernels. A tile is two 32-key halves with the same score registers in turn;
+// the first half's dQ products are issued under the second one's exponentials.
 template <int D, bool kDrop>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2 : 1))) void window_dq_kernel(
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 64 && !kDrop ? 3 : 2))) void window_dq_kernel(
     const bf16_raw* __restrict__ qkv, const bf16_raw* __restrict__ out, const uint8_t* __restrict__ out_rest,
     const bf16_raw* __restrict__ dout, const float* __restrict__ neg_lse_in, float* __restrict__ neg_delta_out,
     bf16_raw* __restrict__ dqkv, Shape s, DropoutParams drop) {
@@ -243,7 +246,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
   constexpr int kDBlocks = D / 32;
   constexpr int kTileBytes = kBN * D * 2;
   constexpr int kAhead = 6;  // fragments in flight
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+  extern __shared__ __attribute__((aligned(256))) char smem[];
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -294,7 +297,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
 #pragma unroll
   for (int ks = 0; ks < kKSteps; ++ks) asm volatile("" ::"v"(__builtin_bit_cast(u32x4, qf[ks])));
   const float c = s.scale * kLog2e;
-  TileAddr<D> at;
+  TileAddrSmall<D> at;
   at.init(lds_addr(smem), lane);
 
   f32x16 dq_acc[kDBlocks];
@@ -308,7 +311,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
     next_tile_ready();
     if (j + 1 < tiles.total) fetch(j + 1);
 
-    if (wave_active && tile_seen(s, key0, q0)) {
+    auto tile = [&](bool masked) {
       // One stream of products: S and dP of the first half (in turn, n odd is dP), of the second half, then dQ of the
       // first half and of the second. Product n's fragment is requested behind product n - kAhead.
       constexpr int kN = 2 * kKSteps, kTN = 2 * kDBlocks, kAll = 2 * kN + 2 * kTN;
@@ -317,42 +320,45 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
       auto request = [&](auto n) {
         if constexpr (n < 2 * kN) {
           constexpr int kb = n / kN, m = n % kN;
-          f[n % kAhead] = read16<(m % 2 ? kTileBytes : 0) + kb * 64 * D>(at.row[m / 2]);
+          f[n % kAhead] = read16<(m % 2 ? kTileBytes : 0) + kb * 64 * D>(at.row(m / 2));
         } else if constexpr (n < kAll) {
           constexpr int m = n - 2 * kN, k = m / kDBlocks, db = m % kDBlocks;  // 16-key step, column block
-          tlo[n % kAhead] = read_tr8<k * 32 * D>(at.tr[db][0]);
-          thi[n % kAhead] = read_tr8<k * 32 * D>(at.tr[db][1]);
+          tlo[n % kAhead] = read_tr8<k * 32 * D>(at.tr(db, 0));
+          thi[n % kAhead] = read_tr8<k * 32 * D>(at.tr(db, 1));
         }
       };
       static_for<0, kAhead>(request);
-      f32x16 s_acc[2], dp_acc[2];
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
+      f32x16 s_acc, dp_acc;  // of the half in hand
+      bf16x8 ds[4];
+      auto start = [&](int kb) {
+        float s0 = neg_lse, dp0 = -delta;
+        asm volatile("" : "+v"(s0), "+v"(dp0));  // (16 copies each are made here, not held through the loop)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          s_acc[kb][i] = neg_lse;
-          dp_acc[kb][i] = -delta;
+          s_acc[i] = s0;
+          dp_acc[i] = dp0;
         }
-      start_masked(s, q_row, q0, key0, h, s_acc);
-      bf16x8 ds[2];
+        if (masked) start_masked(s, q_row, key0 + 32 * kb, h, s_acc);
+      };
       auto multiply = [&](auto n) {
         constexpr int last = n + kAhead - 1 < kAll - 1 ? n + kAhead - 1 : kAll - 1;  // newest request
         constexpr int last1 = last < 2 * kN - 1 ? last : 2 * kN - 1;
         constexpr int younger = (last1 > n ? last1 - n : 0) + 2 * (last >= 2 * kN ? last - (n >= 2 * kN ? n : 2 * kN - 1) : 0);
         if constexpr (n < 2 * kN) {
-          constexpr int kb = n / kN, m = n % kN;
+          constexpr int m = n % kN;
           wait_for<younger>(f[n % kAhead]);
           const bf16x8 a = __builtin_bit_cast(bf16x8, f[n % kAhead]);
-          if constexpr (m % 2 == 0) s_acc[kb] = mfma32(a, qf[m / 2], s_acc[kb]);
-          else dp_acc[kb] = mfma32(a, dof[m / 2], dp_acc[kb]);
+          if constexpr (m % 2 == 0) s_acc = mfma32(a, qf[m / 2], s_acc);
+          else dp_acc = mfma32(a, dof[m / 2], dp_acc);
         } else {
           constexpr int m = n - 2 * kN, k = m / kDBlocks, db = m % kDBlocks;
           wait_for<younger>(tlo[n % kAhead], thi[n % kAhead]);
-          dq_acc[db] = mfma32(join(tlo[n % kAhead], thi[n % kAhead]), ds[k & 1], dq_acc[db]);
+          dq_acc[db] = mfma32(join(tlo[n % kAhead], thi[n % kAhead]), ds[k], dq_acc[db]);
         }
         request(std::integral_constant<int, n + kAhead>{});
+        __builtin_amdgcn_sched_barrier(0);
       };
-      auto prepare = [&](auto kb) {  // dropout, before the elements
+      auto prepare = [&](int kb) {  // dropout, before the elements
         if constexpr (kDrop) {
           uint32_t words[4];
           dropout_words_for_query(drop, bh, q_row, key0 + kb * 32, h, lane, words);
@@ -361,51 +367,44 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const bool keep = ((words[g] >> (8 * e)) & 0xffu) >= drop.threshold;
-              const float dp_true = dp_acc[kb][4 * g + e] + delta;
-              dp_acc[kb][4 * g + e] = (keep ? dp_true * drop.keep_scale : 0.f) - delta;
+              const float dp_true = dp_acc[4 * g + e] + delta;
+              dp_acc[4 * g + e] = (keep ? dp_true * drop.keep_scale : 0.f) - delta;
             }
         }
       };
-      // Elements of a half under product j of `of`: from the third on (the chains' results take that long).
-      auto elements_under = [&](auto kb, auto j, auto of) {
-        if constexpr (j >= 2)
-          static_for<(j - 2) * 16 / (of - 2), (j - 1) * 16 / (of - 2)>(
-              [&](auto i) {
-                constexpr int e = i;
-                s_acc[kb][e] = __builtin_amdgcn_exp2f(s_acc[kb][e] * c) * dp_acc[kb][e];
-              });
+      auto element = [&](auto i) {
+        constexpr int e = i;
+        s_acc[e] = __builtin_amdgcn_exp2f(s_acc[e] * c) * dp_acc[e];
       };
       auto pack_half = [&](auto kb) {
-        const f32x16& a = s_acc[kb];
-        ds[0] = pack_acc8(a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7]);
-        ds[1] = pack_acc8(a[8], a[9], a[10], a[11], a[12], a[13], a[14], a[15]);
+        const f32x16& a = s_acc;
+        constexpr int at = 2 * kb;
+        ds[at] = pack_acc8(a[0], a[1], a[2], a[3], a[4], a[5], a[6], a[7]);
+        ds[at + 1] = pack_acc8(a[8], a[9], a[10], a[11], a[12], a[13], a[14], a[15]);
       };
-      constexpr std::integral_constant<int, 0> k0{};
-      constexpr std::integral_constant<int, 1> k1{};
-      constexpr std::integral_constant<int, kN> of_n{};
-      constexpr std::integral_constant<int, kTN> of_tn{};
-      static_for<0, kN>([&](auto n) {
-        multiply(n);
-        __builtin_amdgcn_sched_barrier(0);
-      });
-      prepare(k0);
-      static_for<kN, 2 * kN>([&](auto n) {
-        multiply(n);
-        elements_under(k0, std::integral_constant<int, n - kN>{}, of_n);
-        __builtin_amdgcn_sched_barrier(0);
-      });
-      pack_half(k0);
-      prepare(k1);
+      start(0);
+      __builtin_amdgcn_sched_barrier(0);
+      static_for<0, kN>(multiply);
+      prepare(0);
+      static_for<0, 16>(element);
+      pack_half(std::integral_constant<int, 0>{});
+      __builtin_amdgcn_sched_barrier(0);
+      start(1);
+      __builtin_amdgcn_sched_barrier(0);
+      static_for<kN, 2 * kN>(multiply);
+      prepare(1);
+      // the second half's elements under the first half's dQ, from the third product on (the chains take that long)
       static_for<2 * kN, 2 * kN + kTN>([&](auto n) {
         multiply(n);
-        elements_under(k1, std::integral_constant<int, n - 2 * kN>{}, of_tn);
+        constexpr int j = n - 2 * kN;
+        if constexpr (j >= 2) static_for<(j - 2) * 16 / (kTN - 2), (j - 1) * 16 / (kTN - 2)>(element);
         __builtin_amdgcn_sched_barrier(0);
       });
-      pack_half(k1);
-      static_for<2 * kN + kTN, kAll>([&](auto n) {
-        multiply(n);
-        __builtin_amdgcn_sched_barrier(0);
-      });
+      pack_half(std::integral_constant<int, 1>{});
+      static_for<2 * kN + kTN, kAll>(multiply);
+    };
+    if (wave_active && tile_seen(s, key0, q0)) {  // wave-uniform, both
+      tile(tile_masked(s, key0, q0));
     }
     at.move((j & 1) ? -2 * kTileBytes : 2 * kTileBytes);
   }
