@@ -104,33 +104,54 @@ struct TileAddrSmall {
 
 // Moves 64-row tiles of [rows][D] bf16 (row pitch in bytes) into LDS, swizzled as tile_off: lane p of a wave's
 // load i lands on row 16 wave + i kRows + p / kChunks, slot p % kChunks, and fetches the chunk that belongs there.
+// Rows past `last` are out of the source's range: the hardware fills them with zeros.
 template <int D>
 struct TileLoader {
   static constexpr int kChunks = D / 8, kRows = 64 / kChunks, kLoads = 16 / kRows;
   unsigned pitch;
   unsigned off[kLoads];  // this lane's, for a whole tile
-  __device__ __forceinline__ static unsigned lane_off(int i, int wave, int lane, int last_row, unsigned pitch) {
-    const int row = 16 * wave + i * kRows + lane / kChunks;
-    return (unsigned)min(row, last_row) * pitch + (unsigned)(((lane % kChunks) ^ tile_xor<D>(row)) * 16);
-  }
   __device__ __forceinline__ void init(int64_t row_stride, int wave, int lane) {
     pitch = (unsigned)row_stride * 2u;
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) off[i] = lane_off(i, wave, lane, 63, pitch);
-  }
-  // rows first .. first + 63 of `base`, rows past `last` repeat it
-  __device__ __forceinline__ void load(const bf16_raw* base, int first, int last, char* tile, int wave, int lane) const {
-    typedef __attribute__((address_space(3))) void lds_ptr_t;
-    const int left = min(last - first, 63);  // >= 0
-    const char* start = reinterpret_cast<const char*>(base) + int64_t(first) * pitch;  // wave-uniform
-    const auto src = __builtin_amdgcn_make_buffer_rsrc((void*)start, 0, (int)((unsigned)left * pitch + 2u * D), 0x00027000);
-    char* dst = tile + 16 * wave * 2 * D;
-#pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      unsigned at = off[i];
-      if (left < 63) at = lane_off(i, wave, lane, left, pitch);  // wave-uniform
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (lds_ptr_t*)(dst + i * kRows * 2 * D), 16, (int)at, 0, 0, 0);
+      const int row = 16 * wave + i * kRows + lane / kChunks;
+      off[i] = (unsigned)row * pitch + (unsigned)(((lane % kChunks) ^ tile_xor<D>(row)) * 16);
     }
+  }
+  // rows first .. first + 63 of `base` (a negative `last`: none, all zeros)
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t aim(const bf16_raw* base, int first, int last) const {
+    const int left = min(last - first, 63);
+    const char* start = reinterpret_cast<const char*>(base) + int64_t(first) * pitch;  // wave-uniform
+    return __builtin_amdgcn_make_buffer_rsrc((void*)start, 0, left < 0 ? 0 : (int)((unsigned)left * pitch + 2u * D), 0x00027000);
+  }
+  template <int I>
+  __device__ __forceinline__ void load_one(__amdgpu_buffer_rsrc_t src, char* tile, int wave) const {
+    typedef __attribute__((address_space(3))) void lds_ptr_t;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(src, (lds_ptr_t*)(tile + 16 * wave * 2 * D + I * kRows * 2 * D), 16, (int)off[I], 0, 0, 0);
+  }
+  __device__ __forceinline__ void load(const bf16_raw* base, int first, int last, char* tile, int wave) const {
+    const auto src = aim(base, first, last);
+    static_for<0, kLoads>([&](auto i) { load_one<i>(src, tile, wave); });
+  }
+};
+
+// The next tile's two loads (K and V, or Q and dO) of a wave, one at a time between the products: a burst of them
+// would keep the wave from issuing products for as long as the loads' addresses take (500 cycles at D = 128).
+template <int D>
+struct NextTile {
+  static constexpr int kLoads = 2 * TileLoader<D>::kLoads;
+  __amdgpu_buffer_rsrc_t a, b;
+  char* dst;
+  template <int I>
+  __device__ __forceinline__ void load_one(const TileLoader<D>& la, const TileLoader<D>& lb, int wave) const {
+    constexpr int kHalf = TileLoader<D>::kLoads;
+    if constexpr (I < kHalf) la.template load_one<I>(a, dst, wave);
+    else if constexpr (I < kLoads) lb.template load_one<I - kHalf>(b, dst + kBN * D * 2, wave);
+  }
+  // behind product n: every other one from the first on
+  template <int N>
+  __device__ __forceinline__ void behind(const TileLoader<D>& la, const TileLoader<D>& lb, int wave) const {
+    if constexpr (N % 2 == 0 && N / 2 < kLoads) load_one<N / 2>(la, lb, wave);
   }
 };
 

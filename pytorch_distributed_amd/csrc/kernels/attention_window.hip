@@ -83,12 +83,13 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
 
   TileLoader<D> loader;
   loader.init(tok_stride, wave, lane);
-  auto fetch = [&](int i) {
-    char* buf = smem + (i & 1) * 2 * kTileBytes;
-    loader.load(k_base, tiles[i] * kBN, T - 1, buf, wave, lane);
-    loader.load(v_base, tiles[i] * kBN, T - 1, buf + kTileBytes, wave, lane);
+  loader.load(k_base, tiles[0] * kBN, T - 1, smem, wave);
+  loader.load(v_base, tiles[0] * kBN, T - 1, smem + kTileBytes, wave);
+  auto following = [&](int j) {  // tile j + 1 (behind the last: nothing)
+    const bool more = j + 1 < tiles.total;
+    const int first = tiles[more ? j + 1 : j] * kBN, last = more ? T - 1 : -1;
+    return NextTile<D>{loader.aim(k_base, first, last), loader.aim(v_base, first, last), smem + ((j + 1) & 1) * 2 * kTileBytes};
   };
-  fetch(0);
   bf16x8 qf[kKSteps];
 #pragma unroll
   for (int ks = 0; ks < kKSteps; ++ks)
@@ -111,7 +112,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
   for (int j = 0; j < tiles.total; ++j) {
     const int key0 = tiles[j] * kBN;
     next_tile_ready();
-    if (j + 1 < tiles.total) fetch(j + 1);
+    const NextTile<D> next = following(j);
 
     if (wave_active && tile_seen(s, key0, q0)) {
       u32x4 kf[kAhead];
@@ -134,6 +135,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
         wait_for<(kN - 1 - n < kAhead - 1 ? kN - 1 - n : kAhead - 1)>(kf[n % kAhead]);
         s_acc[kb] = mfma32(__builtin_bit_cast(bf16x8, kf[n % kAhead]), qf[ks], s_acc[kb]);
         if constexpr (n + kAhead < kN) request(std::integral_constant<int, n + kAhead>{});
+        next.template behind<n>(loader, loader, wave);
         __builtin_amdgcn_sched_barrier(0);
       });
       // the first V fragments travel under the softmax
@@ -206,9 +208,12 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
         if constexpr (n + kAheadV < kVN) request_v(std::integral_constant<int, n + kAheadV>{});
         __builtin_amdgcn_sched_barrier(0);
       });
+    } else {
+      static_for<0, NextTile<D>::kLoads>([&](auto i) { next.template load_one<i>(loader, loader, wave); });
     }
     at.move((j & 1) ? -2 * kTileBytes : 2 * kTileBytes);
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load to LDS outlives the workgroup
 
   const float l_tot = lane_pair_sum(l_run);
   if (q_row < T) {
@@ -268,12 +273,13 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
 
   TileLoader<D> loader;
   loader.init(tok_stride, wave, lane);
-  auto fetch = [&](int i) {
-    char* buf = smem + (i & 1) * 2 * kTileBytes;
-    loader.load(k_base, tiles[i] * kBN, T - 1, buf, wave, lane);
-    loader.load(v_base, tiles[i] * kBN, T - 1, buf + kTileBytes, wave, lane);
+  loader.load(k_base, tiles[0] * kBN, T - 1, smem, wave);
+  loader.load(v_base, tiles[0] * kBN, T - 1, smem + kTileBytes, wave);
+  auto following = [&](int j) {  // tile j + 1 (behind the last: nothing)
+    const bool more = j + 1 < tiles.total;
+    const int first = tiles[more ? j + 1 : j] * kBN, last = more ? T - 1 : -1;
+    return NextTile<D>{loader.aim(k_base, first, last), loader.aim(v_base, first, last), smem + ((j + 1) & 1) * 2 * kTileBytes};
   };
-  fetch(0);
   bf16x8 qf[kKSteps], dof[kKSteps];
   float dpart = 0.f;
   {
@@ -309,7 +315,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
   for (int j = 0; j < tiles.total; ++j) {
     const int key0 = tiles[j] * kBN;
     next_tile_ready();
-    if (j + 1 < tiles.total) fetch(j + 1);
+    const NextTile<D> next = following(j);
 
     auto tile = [&](bool masked) {
       // One stream of products: S and dP of the first half (in turn, n odd is dP), of the second half, then dQ of the
@@ -356,6 +362,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
           dq_acc[db] = mfma32(join(tlo[n % kAhead], thi[n % kAhead]), ds[k], dq_acc[db]);
         }
         request(std::integral_constant<int, n + kAhead>{});
+        next.template behind<n>(loader, loader, wave);
         __builtin_amdgcn_sched_barrier(0);
       };
       auto prepare = [&](int kb) {  // dropout, before the elements
@@ -405,9 +412,12 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
     };
     if (wave_active && tile_seen(s, key0, q0)) {  // wave-uniform, both
       tile(tile_masked(s, key0, q0));
+    } else {
+      static_for<0, NextTile<D>::kLoads>([&](auto i) { next.template load_one<i>(loader, loader, wave); });
     }
     at.move((j & 1) ? -2 * kTileBytes : 2 * kTileBytes);
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load to LDS outlives the workgroup
 
   if (q_row < T) {
     bf16_raw* dq_row = dqkv + (int64_t(b) * T + q_row) * tok_stride + int64_t(head) * D;

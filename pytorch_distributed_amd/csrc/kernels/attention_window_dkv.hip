@@ -127,17 +127,21 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
   TileLoader<D> q_loader, do_loader;
   q_loader.init(tok_stride, wave, lane);
   do_loader.init(o_stride, wave, lane);
-  auto fetch = [&](int tile, int buf) {
+  auto fetch_constants = [&](int tile, int buf) {
     typedef __attribute__((address_space(1))) const void global_ptr_t;
     typedef __attribute__((address_space(3))) void lds_ptr_t;
-    char* dst = smem + buf * 2 * kTileBytes;
-    q_loader.load(q_base, tile * kBN, T - 1, dst, wave, lane);
-    do_loader.load(do_base, tile * kBN, T - 1, dst + kTileBytes, wave, lane);
     if (wave < 2) {  // wave 0: -lse / c, wave 1: -delta of the tile's 64 queries
       const float* src = (wave == 0 ? lse_row : delta_row) + min(tile * kBN + lane, T - 1);
       __builtin_amdgcn_global_load_lds((global_ptr_t*)src, (lds_ptr_t*)(row_smem + buf * 512 + wave * 256), 4, 0, 0);
     }
   };
+  auto fetch = [&](int tile, int buf) {
+    char* dst = smem + buf * 2 * kTileBytes;
+    q_loader.load(q_base, tile * kBN, T - 1, dst, wave);
+    do_loader.load(do_base, tile * kBN, T - 1, dst + kTileBytes, wave);
+    fetch_constants(tile, buf);
+  };
+  [[maybe_unused]] NextTile<D> following;  // what the stream of both sub-tiles loads on its way
   if constexpr (!kFar) fetch(first_tile, 0);
   bf16x8 kf[kKSteps], vf[kKSteps];
 #pragma unroll
@@ -251,6 +255,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
     }
     if constexpr (subs == 2 && n == kN - kAhead) request_constants(std::integral_constant<int, 1>{});
     request(subs, std::integral_constant<int, n + kAhead>{});
+    if constexpr (subs == 2) following.template behind<n>(q_loader, do_loader, wave);
   };
   constexpr std::integral_constant<int, 0> s0{};
   constexpr std::integral_constant<int, 1> s1{};
@@ -365,7 +370,14 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
   for (int j = first_tile; j < end_tile; ++j) {
     const int buf = (j - first_tile) & 1;
     next_tile_ready();
-    if (j + 1 < end_tile) fetch(j + 1, buf ^ 1);
+    if constexpr (kDrop) {
+      if (j + 1 < end_tile) fetch(j + 1, buf ^ 1);
+    } else {
+      const bool more = j + 1 < end_tile;
+      const int first = (more ? j + 1 : j) * kBN, last = more ? T - 1 : -1;
+      if (more) fetch_constants(j + 1, buf ^ 1);
+      following = NextTile<D>{q_loader.aim(q_base, first, last), do_loader.aim(do_base, first, last), smem + (buf ^ 1) * 2 * kTileBytes};
+    }
     const int q0 = j * kBN;
     const int next = buf ? -2 * kTileBytes : 2 * kTileBytes;
     if constexpr (kDrop) {  // (the pipelined form has no registers left for its masks)
@@ -382,6 +394,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
     }
   }
 
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load to LDS outlives the workgroup
   if constexpr (D == 128) settle(dk_acc), settle(dv_acc);
   if (key < T) {
     bf16_raw* dk_row = dqkv + (int64_t(b) * T + key) * tok_stride + int64_t(s.H) * D + int64_t(head) * D;
