@@ -45,6 +45,7 @@ namespace pda {
 namespace {
 
 typedef __attribute__((ext_vector_type(8))) int i32x8;
+typedef u32x4 __attribute__((aligned(2))) u32x4_anywhere;  // 16 bytes of global memory at any alignment
 
 constexpr int kThreads = 256;
 constexpr int kStages = 4;
@@ -110,7 +111,7 @@ struct Problem {
   Operand x, w;
   void* out;         // [M, N] (bf16 or fp32), or the fp32 partials [slices][M][N]
   const void* bias;  // [N] or null
-  bool out_f32, bias_f32, vec;  // vec: rows are 16-byte aligned
+  bool out_f32, bias_f32;
   int steps, steps_per_slice, tasks;
 };
 
@@ -436,7 +437,7 @@ __global__ __launch_bounds__(kThreads) void fp8_gemm_kernel(const Problems P) {
       int el = lane;
       asm volatile("" : "+v"(el));  // (addresses are formed here, not held through the products)
       const int er = el & 31, eh = el >> 5;
-      const int vec = __builtin_amdgcn_readfirstlane(pr.vec), bias_f32 = __builtin_amdgcn_readfirstlane(pr.bias_f32);
+      const int bias_f32 = __builtin_amdgcn_readfirstlane(pr.bias_f32);
       const int has_bias = __builtin_amdgcn_readfirstlane(pr.bias != nullptr);  // (held: not fetched after every store)
       auto store_quarter = [&](auto out_f32) {
         using Out = std::conditional_t<decltype(out_f32)::value, float, bf16_raw>;
@@ -470,7 +471,9 @@ __global__ __launch_bounds__(kThreads) void fp8_gemm_kernel(const Problems P) {
             }
           }
           const int col = n0 + 32 * (kWB * wj + b0) + (el & 7) * kVec;
-          const unsigned at0 = col < N ? ((unsigned)(32 * kWB * wi + (el >> 3)) * (unsigned)N + (unsigned)col) * kSize : 0x80000000u;
+          const unsigned row0 = (unsigned)(32 * kWB * wi + (el >> 3)) * (unsigned)N * kSize;
+          const unsigned at0 = col + kVec <= N ? row0 + (unsigned)col * kSize : 0x80000000u;
+          const bool ragged = N % kVec != 0 && n0 + 32 * (kWB * wj + b0 + kB) > N;
           using Piece = std::conditional_t<kSize == 2, u32x2, f32x4>;  // four features of a token
           Piece piece[kB][4];
           auto round_up = [&](int a) {  // one block at a time leaves the accumulator file
@@ -506,17 +509,16 @@ __global__ __launch_bounds__(kThreads) void fp8_gemm_kernel(const Problems P) {
             w[3] = chunk_read<3072>(from);
             if (a + 1 < kWB) round_up(a + 1);  // while they come
             asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3])::"memory");
-            // out of range (rows past M, columns past N): dropped, but issued and counted
-            if (vec) {
+            // Rows at any alignment. Out of range (rows past M, pieces past or across N): dropped, but issued and counted.
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              __builtin_amdgcn_raw_buffer_store_b128(w[i], dst, (int)(at0 + (unsigned)((32 * a + 8 * i) * N) * kSize), 0, 0);
+            if (ragged) {  // wave-uniform: the piece across N, one element at a time
 #pragma unroll
               for (int i = 0; i < 4; ++i)
-                __builtin_amdgcn_raw_buffer_store_b128(w[i], dst, (int)(at0 + (unsigned)((32 * a + 8 * i) * N) * kSize), 0, 0);
-            } else {  // rows at any alignment: one element at a time
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int e = 0; e < kVec; ++e) {
-                  const unsigned to = col + e < N ? at0 + (unsigned)((32 * a + 8 * i) * N + e) * kSize : 0x80000000u;
+                for (int e = 0; e + 1 < kVec; ++e) {
+                  const unsigned to = col + kVec > N && col + e < N ? row0 + (unsigned)((32 * a + 8 * i) * N + col + e) * kSize : 0x80000000u;
                   if constexpr (kSize == 4) __builtin_amdgcn_raw_buffer_store_b32(w[i][e], dst, (int)to, 0, 0);
                   else __builtin_amdgcn_raw_buffer_store_b16((unsigned short)(w[i][e / 2] >> (16 * (e & 1))), dst, (int)to, 0, 0);
                 }
@@ -559,23 +561,22 @@ __global__ __launch_bounds__(kThreads) void fp8_gemm_kernel(const Problems P) {
             }
           }
         __syncthreads();
-        if (pr.vec) {
-          const int ch = threadIdx.x % kChunks, n = n0 + ch * kVec;
-          if (n < N) {  // (rows are whole chunks here)
+        const int ch = threadIdx.x % kChunks, n = n0 + ch * kVec;
+        if (n < N) {
 #pragma unroll 4
-            for (int q = threadIdx.x / kChunks; q < kTile; q += kThreads / kChunks) {
-              const u32x4 w = *reinterpret_cast<const u32x4*>(smem + q * kRowBytes + ((ch ^ (q & 31 & (kChunks - 1))) * 16));
-              if (m0 + q < M) *reinterpret_cast<u32x4*>(out + int64_t(m0 + q) * N + n) = w;
-            }
-          }
-        } else {  // rows at any alignment: an element per lane, neighbours in neighbouring lanes
-          const int col = threadIdx.x % kTile, n = n0 + col;
-          if (n < N) {
-#pragma unroll 4
-            for (int q = threadIdx.x / kTile; q < kTile; q += kThreads / kTile) {
-              const Out w = *reinterpret_cast<const Out*>(smem + q * kRowBytes + (((col / kVec) ^ (q & 31 & (kChunks - 1))) * 16) +
-                                                          (col % kVec) * (int)sizeof(Out));
-              if (m0 + q < M) out[int64_t(m0 + q) * N + n] = w;
+          for (int q = threadIdx.x / kChunks; q < kTile; q += kThreads / kChunks) {
+            const u32x4 w = *reinterpret_cast<const u32x4*>(smem + q * kRowBytes + ((ch ^ (q & 31 & (kChunks - 1))) * 16));
+            if (m0 + q >= M) break;
+            Out* to = out + int64_t(m0 + q) * N + n;
+            if (n + kVec <= N) {
+              *reinterpret_cast<u32x4_anywhere*>(to) = w;
+            } else {
+#pragma unroll
+              for (int e = 0; e + 1 < kVec; ++e)
+                if (n + e < N) {
+                  if constexpr (sizeof(Out) == 4) to[e] = __uint_as_float(w[e]);
+                  else to[e] = (bf16_raw)(w[e / 2] >> (16 * (e & 1)));
+                }
             }
           }
         }
@@ -796,7 +797,6 @@ void fp8_gemm(const Fp8GemmProblem* problems, int n, const Fp8ColumnSums* sums, 
     void* out = fold ? (void*)g.partial : g.out;
     const int64_t tasks = ceil_div(M, g.plan.tile) * ceil_div(N, g.plan.tile) * g.plan.slices;
     ps[i] = Problem{operand(g.x), operand(g.w), out, fold ? nullptr : g.bias, f32, g.bias_dtype == kF32,
-                    (int64_t(N) * (f32 ? 4 : 2)) % 16 == 0 && reinterpret_cast<uintptr_t>(out) % 16 == 0,
                     g.K / kStageK, g.plan.steps_per_slice, (int)tasks};
     if (fold)
       add_fold(Fold{g.partial, g.bias, g.out, int64_t(M) * N, g.plan.slices, N, 0, g.bias_dtype == kF32, g.out_dtype == kF32,
