@@ -106,7 +106,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
   for (int i = 0; i < kDBlocks; ++i)
 #pragma unroll
     for (int j = 0; j < 16; ++j) o_acc[i][j] = 0.f;
-  float m_run = -INFINITY, l_run = 0.f;  // running row maximum (exp2 units), this lane's share of the row sum
+  float m_run = -INFINITY, l_run = 0.f;  // running reference of the row (exp2 units), this lane's share of the row sum
   const float c = s.scale * kLog2e;
 
   for (int j = 0; j < tiles.total; ++j) {
@@ -158,8 +158,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
       }
       float mx = fmaxf(m0, m1);
       mx = c * lane_pair_max(mx);
-      const float m_new = fmaxf(m_run, mx);  // finite: the wave's first tile holds every row's own key
-      const bool grew = m_new > m_run;
+      // A row's reference moves only when its maximum has outgrown it by 2^8: probabilities up to 256 times the
+      // reference's cost no precision, and most tiles are spared the pass over the accumulators (with 32 rows to a
+      // wave, nearly every tile has some row with a new maximum).
+      const bool grew = mx > m_run + 8.f;
+      const float m_new = grew ? mx : m_run;  // finite: the wave's first tile holds every row's own key
       const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
       m_run = m_new;
       float psum0 = 0.f, psum1 = 0.f;
