@@ -180,7 +180,7 @@ def _reference_backward(dy2, weight, x2, need_x, need_w, need_b):
 class _Fp8LinearFn(torch.autograd.Function):
     """The layer where a Python object takes part: a gradient goes straight into its owner's buffer (gradient
     sink, see ops.linear), or ``x`` is rebuilt from a recipe; and the reference path. (Otherwise the extension's
-    own node runs: the same computation with a third of the host time.)"""
+    own node runs: the same computation with two thirds of the host time.)"""
 
     @staticmethod
     def forward(ctx, x, weight, bias, regen):
