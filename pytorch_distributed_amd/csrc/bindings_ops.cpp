@@ -683,7 +683,9 @@ void check_fp8_source(const at::Tensor& x, const char* name) {
 
 // `x` [..., C] as a matrix [rows, C] that check_fp8_source accepts, copied only if it has to be.
 at::Tensor fp8_source(const at::Tensor& x) {
-  at::Tensor m = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
+  int64_t rows = 1;
+  for (int64_t i = 0; i + 1 < x.dim(); ++i) rows *= x.size(i);
+  at::Tensor m = x.dim() == 2 ? x : x.reshape({rows, x.size(-1)});
   const bool ok = (m.size(1) <= 1 || m.stride(1) == 1) && (m.size(0) <= 1 || m.stride(0) >= m.size(1));
   return ok ? m : m.contiguous();
 }

@@ -30,6 +30,7 @@ CPU tensors and ``PDA_FORCE_REFERENCE=1`` run the PyTorch references below, the 
 """
 from __future__ import annotations
 
+import math
 from typing import Optional, Tuple, Union
 
 import torch
@@ -166,6 +167,10 @@ def fp8_matmul(a: Fp8Matrix, b: Fp8Matrix, bias: Optional[torch.Tensor] = None,
 
 
 # --------------------------------------------------------------------------- the layer
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    return x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
+
+
 def _reference_backward(dy2, weight, x2, need_x, need_w, need_b):
     dx = dw = db = None
     if need_x:
@@ -193,7 +198,7 @@ class _Fp8LinearFn(torch.autograd.Function):
         if ctx.hip:
             y, *kept = _ext.require().fp8_linear_forward(x, weight, bias, keep)
         else:
-            x2 = x.reshape(-1, x.shape[-1])
+            x2 = _rows(x)
             y = fp8_matmul_reference(quantize_fp8_reference(x2), quantize_fp8_reference(weight, "tiles")[0], bias, x.dtype)
             y = y.view(*x.shape[:-1], weight.shape[0])
             kept = [x2] if keep else []
@@ -215,8 +220,8 @@ class _Fp8LinearFn(torch.autograd.Function):
             x = ctx.regen.rebuild(*[None if missing else next(it) for missing in ctx.regen_none])
         if not ctx.hip:
             if need_w:
-                x = kept[0] if x is None else x.reshape(-1, x.shape[-1])
-            dx, dw, db = _reference_backward(dy.reshape(-1, dy.shape[-1]), weight, x, need_x, need_w, need_b)
+                x = kept[0] if x is None else _rows(x)
+            dx, dw, db = _reference_backward(_rows(dy), weight, x, need_x, need_w, need_b)
             return (None if dx is None else dx.view(ctx.x_shape)), dw, db, None
         w_sink, b_sink = ctx.sinks
         w_target = w_sink() if need_w and w_sink is not None else None

@@ -134,6 +134,16 @@ def test_linear_few_tokens(tokens):
     assert torch.equal(b.grad, torch.full((8,), float(tokens)))
 
 
+@pytest.mark.parametrize("shape,out", [((2, 3, 0), 8), ((2, 3, 16), 0), ((2, 0, 16), 8), ((0, 3, 0), 4)])
+def test_linear_without_elements(shape, out):
+    x, w, b = torch.randn(shape, requires_grad=True), torch.randn(out, shape[-1], requires_grad=True), torch.ones(out, requires_grad=True)
+    y = ops.fp8_linear(x, w, b)
+    assert torch.equal(y, torch.ones(*shape[:-1], out))
+    y.sum().backward()
+    assert x.grad.shape == x.shape and not x.grad.any() and w.grad.shape == w.shape and not w.grad.any()
+    assert torch.equal(b.grad, torch.full((out,), float(shape[0] * shape[1])))
+
+
 def test_refusals():
     x = torch.randn(4, 16)
     w = torch.randn(8, 16)

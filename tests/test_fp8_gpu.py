@@ -239,6 +239,52 @@ def test_layer_empty_and_strided():
         assert all(torch.equal(i, j) for i, j in zip(a, c))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape,out", [((2, 3, 0), 8), ((2, 3, 16), 0), ((2, 0, 16), 8), ((0, 3, 0), 4)])
+def test_layer_without_elements(shape, out, dtype):
+    make = lambda *s: torch.ones(s, device=DEV, dtype=dtype).requires_grad_()  # noqa: E731
+    x, w, b = make(*shape), make(out, shape[-1]), make(out)
+    y = ops.fp8_linear(x, w, b)
+    assert y.shape == (*shape[:-1], out) and (y == (1.0 + shape[-1])).all()
+    y.sum().backward()
+    assert x.grad.shape == x.shape and (x.grad == out).all() and w.grad.shape == w.shape and (w.grad == shape[0] * shape[1]).all()
+    assert (b.grad == shape[0] * shape[1]).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(0, 5, 200), (7, 0, 200), (7, 5, 0), (0, 0, 0)])
+def test_product_without_elements(m, n, k):
+    a, b = ops.quantize_fp8(torch.ones(m, k, device=DEV)), ops.quantize_fp8(torch.ones(n, k, device=DEV))
+    c = torch.arange(n, device=DEV, dtype=torch.float32)
+    for dtype in (torch.bfloat16, torch.float32):
+        y = ops.fp8_matmul(a, b, c, dtype)
+        assert y.dtype == dtype and torch.equal(y.float(), (c + k).expand(m, n))
+
+
+def test_no_second_derivative():
+    x, w, b, dy = layer_case(20, 30, 40, torch.bfloat16)
+    y = ops.fp8_linear(x, w, b)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(y, [x], dy, create_graph=True)
+
+
+def test_two_graphs_in_turn():
+    """Two captured layers, replayed in turn and beside each other's eager form: neither uses the other's workspace."""
+    made = []
+    for m, n, k in ((700, 256, 384), (130, 1000, 2600)):
+        x, w, b, dy = layer_case(m, n, k, torch.bfloat16)
+        want = [t.clone() for t in torch.autograd.grad(ops.fp8_linear(x, w, b), [x, w, b], dy)]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = torch.autograd.grad(ops.fp8_linear(x, w, b), [x, w, b], dy)
+        made.append((graph, got, want, (x, w, b, dy)))
+    for _ in range(3):
+        for graph, *_ in made:
+            graph.replay()
+        for _, got, want, (x, w, b, dy) in made:
+            assert all(torch.equal(i, j) for i, j in zip(got, want))
+            assert all(torch.equal(i, j) for i, j in zip(torch.autograd.grad(ops.fp8_linear(x, w, b), [x, w, b], dy), want))
+
+
 def test_side_stream_and_graph():
     x, w, b, dy = layer_case(512, 256, 384, torch.bfloat16)
     want = [t.clone() for t in (lambda y: (y.detach(), *torch.autograd.grad(y, [x, w, b], dy)))(ops.fp8_linear(x, w, b))]

@@ -96,6 +96,21 @@ def test_large_scores():
 
 
 @pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("slope", [-0.2, -0.05, -0.01, 0.01, 0.2])
+def test_scores_that_grow_from_tile_to_tile(D, slope):
+    """Scores rise or fall steadily with the key's age, a little or a lot per tile, and reach some 120."""
+    T, window, sinks = 600, 500, 70
+    qkv, dout = inputs(1, T, 1, D, seed=21, size=0.05)
+    v = qkv.view(1, T, 3, D)
+    v[:, :, 0, 0], v[:, :, 1, 0] = 1.0, slope * math.sqrt(D) * torch.arange(T, device=DEV)
+    v[:, :, 2] *= 20.0
+    out, g = run(qkv, dout, 1, window, sinks)
+    want, tol, wg, tg = oracle(qkv, dout, 1, window, sinks)
+    check(out, want, tol)
+    check(g, wg, tg)
+
+
+@pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("window,sinks", [(50, 3), (150, 40)])
 def test_dropout(D, window, sinks):
     B, T, H, p, seed = 2, 300, 2, 0.25, 1234
@@ -175,6 +190,32 @@ def test_side_stream_and_graph():
         eager = run(qkv * (1 + 0.25 * k), dout * (k + 1), H, window, sinks)
         assert torch.equal(out, eager[0]) and torch.equal(g, eager[1]), k
         torch.cuda.synchronize()
+
+
+def test_no_second_derivative():
+    qkv, dout = inputs(1, 70, 1, 64)
+    leaf = qkv.requires_grad_()
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(ops.window_attention(leaf, 1, 20), leaf, dout, create_graph=True)
+
+
+def test_two_graphs_in_turn():
+    made = []
+    for T, H, D, window, sinks in ((900, 2, 64, 100, 4), (500, 3, 128, 64, 70)):
+        qkv, dout = inputs(1, T, H, D, seed=T)
+        want = run(qkv, dout, H, window, sinks)
+        leaf = qkv.detach().clone().requires_grad_()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.window_attention(leaf, H, window, sinks)
+            (g,) = torch.autograd.grad(out, leaf, dout)
+        made.append((graph, (out, g), want, (qkv, dout, H, window, sinks)))
+    for _ in range(3):
+        for graph, *_ in made:
+            graph.replay()
+        for _, got, want, args in made:
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+            assert all(torch.equal(a, b) for a, b in zip(run(*args), want))
 
 
 def test_empty_batch_and_refusals():
