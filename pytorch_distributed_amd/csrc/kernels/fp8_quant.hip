@@ -19,8 +19,11 @@
 //
 // What bounds it: memory. A workgroup owns a 128 x 128 tile held in registers (8 rows x 8 columns per
 // thread), so x is read once for both layouts; the transposed bytes pass through a swizzled 16 KiB LDS
-// tile and leave as whole 128-byte lines. Measured: 65536 x 5120 bf16 to both layouts 306 us = 4.4 TB/s, 6400 x 1600
-// fp32 by tiles 12.7 us = 4.8 TB/s (a large copy reaches 5.1); a small matrix costs its launch, 7 us.
+// tile and leave as whole 128-byte lines. Measured: 65536 x 5120 bf16 to both layouts 288 us = 4.7 TB/s, 6400 x 1600
+// fp32 by tiles 12.7 us = 4.8 TB/s (a large copy reaches 5.1); a small matrix costs its launch, 7 us. bf16 values stay
+// packed in registers: eight workgroups on a compute unit instead of five (306 -> 288; 8192 x 5120 54 -> 46).
+#include <type_traits>
+
 #include "common.h"
 #include "pda_kernels.h"
 
@@ -53,30 +56,63 @@ __device__ __forceinline__ float finite_abs(float x) {
   return a < kInf ? a : 0.f;
 }
 
+// Eight values of one row, as they are kept: bf16 pairs (half the registers, so eight workgroups fit a compute unit
+// where five would), or floats.
+template <typename T>
+struct Eight;
+template <>
+struct Eight<bf16_raw> {
+  u32x4 w;
+  __device__ __forceinline__ float operator[](int k) const { return k & 1 ? bf16_hi(w[k / 2]) : bf16_lo(w[k / 2]); }
+  __device__ __forceinline__ void forget() { asm volatile("" : "+v"(w)); }  // unpacked again from here on, not held
+};
+template <>
+struct Eight<float> {
+  f32x4 a, b;
+  __device__ __forceinline__ float operator[](int k) const { return k < 4 ? a[k & 3] : b[k & 3]; }
+  __device__ __forceinline__ void forget() {}
+};
+
 // Eight values of one row starting at column c (c % 8 == 0); columns >= C and rows >= R read as zeros. Rows lie at
 // any multiple of a value: global memory takes 16-byte accesses at any alignment (41160 x 2374 bf16 by columns, rows
-// at multiples of 4 bytes: 156 us value by value, 86 so).
+// at multiples of 4 bytes: 156 us value by value, 70 so).
 typedef u32x4 __attribute__((aligned(2))) u32x4_anywhere;
 typedef f32x4 __attribute__((aligned(4))) f32x4_anywhere;
 template <typename T>
-__device__ __forceinline__ void load8(const T* __restrict__ x, int64_t ld, int R, int C, int row, int c, float (&v)[8]) {
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = 0.f;
-  if (row >= R || c >= C) return;
+__device__ __forceinline__ Eight<T> load8(const T* __restrict__ x, int64_t ld, int R, int C, int row, int c) {
+  Eight<T> v;
+  if constexpr (sizeof(T) == 2) v.w = u32x4{0u, 0u, 0u, 0u};
+  else v.a = v.b = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (row >= R || c >= C) return v;
   const T* p = x + int64_t(row) * ld + c;
   if (c + 8 <= C) {
     if constexpr (sizeof(T) == 2) {
-      VecIO<T>::unpack(*reinterpret_cast<const u32x4_anywhere*>(p), v);
+      v.w = *reinterpret_cast<const u32x4_anywhere*>(p);
     } else {
-      const f32x4 a = *reinterpret_cast<const f32x4_anywhere*>(p), b = *reinterpret_cast<const f32x4_anywhere*>(p + 4);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = a[i], v[4 + i] = b[i];
+      v.a = *reinterpret_cast<const f32x4_anywhere*>(p);
+      v.b = *reinterpret_cast<const f32x4_anywhere*>(p + 4);
     }
-    return;
+    return v;
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (c + i < C) v[i] = VecIO<T>::load1(p + i);
+  for (int i = 0; i < 7; ++i)
+    if (c + i < C) {
+      if constexpr (sizeof(T) == 2) v.w[i / 2] |= uint32_t(p[i]) << (16 * (i & 1));
+      else if (i < 4) v.a[i] = p[i];
+      else v.b[i - 4] = p[i];
+    }
+  return v;
+}
+
+// Maximum over the 16 lanes of a row group, by rotations inside it.
+__device__ __forceinline__ float max16(float m) {
+  auto turned = [](float x, auto by) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x120 + decltype(by)::value, 0xf, 0xf, false));
+  };
+  m = fmaxf(m, turned(m, std::integral_constant<int, 8>{}));
+  m = fmaxf(m, turned(m, std::integral_constant<int, 4>{}));
+  m = fmaxf(m, turned(m, std::integral_constant<int, 2>{}));
+  return fmaxf(m, turned(m, std::integral_constant<int, 1>{}));
 }
 
 // Thread (g = tid / 16, j = tid % 16) holds rows 8 g .. 8 g + 7 and columns 8 j .. 8 j + 7 of the tile.
@@ -93,7 +129,7 @@ struct Matrices {
 };
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void quantize_kernel(const Matrices all) {
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 2 ? 8 : 5))) void quantize_kernel(const Matrices all) {
   __shared__ __attribute__((aligned(16))) uint8_t tile[kBlock * kBlock];
   __shared__ float red[4][kBlock];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -108,9 +144,9 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const Matrices all) 
   const int row0 = rb * kBlock + 8 * g, col0 = cb * kBlock + 8 * j;
   uint8_t *const q = mat.q, *const s = mat.s, *const qt = mat.qt, *const st = mat.st;
 
-  float v[8][8];
+  Eight<T> v[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) load8<T>(x, mat.ld, R, C, row0 + i, col0, v[i]);
+  for (int i = 0; i < 8; ++i) v[i] = load8<T>(x, mat.ld, R, C, row0 + i, col0);
 
   float tile_inv = 1.f;
   uint32_t tile_byte = 0;
@@ -140,6 +176,11 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const Matrices all) 
     }
   }
 
+  auto forget = [&]() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i].forget();
+  };
+  forget();
   if (q) {
     const int64_t Cp = int64_t(n_cb) * kBlock;
     const int pitch = (n_cb + 3) & ~3;
@@ -151,8 +192,7 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const Matrices all) 
         float m = 0.f;
 #pragma unroll
         for (int k = 0; k < 8; ++k) m = fmaxf(m, finite_abs(v[i][k]));
-#pragma unroll
-        for (int off = 8; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+        m = max16(m);
         const uint32_t byte = scale_byte(m);
         inv = inverse_scale(byte);
         if (row < R && j == 0) {
@@ -169,6 +209,7 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const Matrices all) 
     }
   }
 
+  forget();
   if (mat.sums) {  // column sums of this 128-row block: rows in a thread, row groups in a wave, waves in order
     float sum[8];
 #pragma unroll
@@ -188,6 +229,7 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const Matrices all) 
     __syncthreads();
   }
 
+  forget();
   if (qt) {
     float inv[8];
     if (mat.tiles) {
@@ -221,6 +263,7 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const Matrices all) 
         }
       }
     }
+    forget();
     // Column c of the tile is a 128-byte LDS row; its 16-byte chunks are permuted by the column group j
     // (the lanes of a store share the column within their group), so 8 column groups take 8 chunks.
 #pragma unroll
