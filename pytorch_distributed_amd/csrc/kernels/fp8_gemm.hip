@@ -6,15 +6,15 @@
 // takes such a byte per row and applies it inside the instruction, so a block-scaled product costs no
 // vector instruction per product more than an unscaled one.
 //
-// Structure. A workgroup of 4 waves (2 x 2) owns a square output tile, each wave a quarter as kWB x kWB
-// blocks of 32 x 32. A pipeline stage is 64 values of the contraction: [tile rows][64 bytes] of each
+// Structure. A workgroup of 4 waves (2 x 2) owns an output tile of 128 x 128, 256 x 192 or 256 x 256 (tokens x
+// features), each wave a quarter as kA x kB blocks of 32 x 32. A pipeline stage is 64 values of the contraction: [tile rows][64 bytes] of each
 // operand, moved global -> LDS by buffer loads into a ring of four. The body of stage t
 //   * waits until stage t + 1 has landed (counted: two younger stages stay in flight) and meets the
 //     other waves, who by then have read stage t out of LDS;
 //   * issues the products of stage t from registers, and between them the LDS reads of stage t + 1 and
 //     the loads of stage t + 4 into the slot that stage t has left.
-// One barrier per 16 matrix instructions (1,024 matrix cycles) of a wave at kWB = 4.
-// 256 tile (one workgroup per compute unit): a workgroup takes several tiles, and the stages run on across
+// One barrier per 16 matrix instructions (1,024 matrix cycles) of a wave at 256 x 256.
+// Large tiles (one workgroup per compute unit): a workgroup takes several tiles, and the stages run on across
 // them: while a tile is rounded and stored, the next one's first four stages are on their way. Measured against
 // a workgroup per tile: 8192 x 5120 x 1280 (640 tiles) 84 -> 72 us, 8192 x 22016 x 4096 (2,752) 665 -> 591.
 // What bounds it: the matrix pipes at the clock that the power leaves. 8192 x 22016 x 4096 runs at 2,500 TFLOP/s
@@ -31,7 +31,7 @@
 // bits: measured (random e4m3 operands) up to 1.3e-4 of sum |x w|, 5e-5 in norm, whatever the contraction's
 // length. Next to a bf16 result's rounding (1.7e-3) that is nothing; an fp32 result is computed with kWide
 // instead: fragments widened to bf16 on the way to v_mfma_f32_32x32x16_bf16, scale included (exact), whose
-// sums are good to 6e-8, at half the matrix rate (1003 x 1601 x 777: 14.4 us).
+// sums are good to 6e-8, at half the matrix rate (1003 x 1601 x 777: 12.1 us).
 //
 // Few output tiles (weight gradients, few tokens): the contraction is cut into slices of whole 512-value
 // scale groups, fp32 partial tiles are folded in slice order by a second kernel (deterministic).
@@ -129,7 +129,7 @@ struct Place {
 // (whoever had a long task then gets a short one). Within a round, and within a problem, the 8 XCDs get contiguous
 // ranges; consecutive tasks walk kGroupM token tiles x all feature tiles, so an XCD's workgroups share operand
 // rows in its L2.
-template <int kTile>
+template <int kTileM, int kTileN>
 __device__ __forceinline__ Place place_of(const Problems& P, int w, int grid, int round) {
   const int base = round * grid, left = P.p[0].tasks + P.p[1].tasks - base;
   const int count = min(grid, left);
@@ -143,7 +143,7 @@ __device__ __forceinline__ Place place_of(const Problems& P, int w, int grid, in
   const int q8 = n / 8, r8 = n % 8, x = j % 8;
   const int task = base + (second ? c0 - P.p[0].tasks : 0) + (x < r8 ? x * (q8 + 1) : r8 * (q8 + 1) + (x - r8) * q8) + j / 8;
   const Problem& pr = P.p[second];
-  const int tiles_m = (pr.x.rows + kTile - 1) / kTile, tiles_n = (pr.w.rows + kTile - 1) / kTile;
+  const int tiles_m = (pr.x.rows + kTileM - 1) / kTileM, tiles_n = (pr.w.rows + kTileN - 1) / kTileN;
   const int n_tiles = tiles_m * tiles_n;
   const int slice = task / n_tiles;
   const int tile = task - slice * n_tiles;
@@ -152,8 +152,8 @@ __device__ __forceinline__ Place place_of(const Problems& P, int w, int grid, in
   const int group_rows = min(kGroupM, tiles_m - group * kGroupM);
   at.which = second;
   at.slice = slice;
-  at.m0 = (group * kGroupM + in_group % group_rows) * kTile;
-  at.n0 = (in_group / group_rows) * kTile;
+  at.m0 = (group * kGroupM + in_group % group_rows) * kTileM;
+  at.n0 = (in_group / group_rows) * kTileN;
   at.first = slice * pr.steps_per_slice;  // a multiple of kGroupStages
   at.n_steps = min(pr.steps_per_slice, pr.steps - at.first);
   return at;
@@ -161,38 +161,46 @@ __device__ __forceinline__ Place place_of(const Problems& P, int w, int grid, in
 
 constexpr int kScaleRing = 4;  // scale groups in LDS: loads run at most 4 stages ahead, at least 2 stages (one group) a tile
 constexpr int kBiasRing = 4;   // likewise of tiles
-constexpr int kWaveStage = 4096;  // bytes of LDS a wave turns its output around in
 
-constexpr int lds_bytes(int kWB) {
-  const int tile = 64 * kWB;
-  const int ring = kStages * 2 * tile * kStageK, scales = kScaleRing * 2 * tile * 4;
-  return kWB == 4 ? ring + scales + kBiasRing * tile * 4 + 4 * kWaveStage : ring + scales + tile * 4;
+// kA x kB: blocks of 32 tokens x 32 features of a wave; four waves (2 x 2) to a tile.
+constexpr bool streams(int kA) { return kA == 4; }  // several tiles per workgroup, as one stream of stages
+constexpr int wave_turn_bytes(int kB) { return 32 * (kB == 3 ? 192 : 128); }  // LDS a wave turns 32 tokens of its output around in
+constexpr int lds_bytes(int kA, int kB) {
+  const int m = 64 * kA, n = 64 * kB;
+  const int ring = kStages * (m + n) * kStageK, scales = kScaleRing * 2 * m * 4;
+  return streams(kA) ? ring + scales + kBiasRing * n * 4 + 4 * wave_turn_bytes(kB) : ring + scales + n * 4;
 }
 
-template <int kWB, bool kWide>
+// Wait until at most so many vector memory operations of this wave are left.
+template <int kLeft>
+__device__ __forceinline__ void wait_vm() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"i"(kLeft) : "memory");
+}
+
+template <int kA, int kB, bool kWide>
 __global__ __launch_bounds__(kThreads) void fp8_gemm_kernel(const Problems P) {
-  constexpr bool kStream = kWB == 4;           // several tiles per workgroup, as one stream of stages
-  constexpr int kTile = 64 * kWB;
-  constexpr int kSlab = kTile * kStageK;       // bytes of one operand's stage
-  constexpr int kStageBytes = 2 * kSlab;
-  constexpr int kPieces = kTile / 64;          // 16-row loads per wave, stage and operand
-  constexpr int kLoads = 2 * kPieces;          // per wave and stage
-  constexpr int kScaleLoads = kTile / 128;     // 64-row scale loads per wave and group (both operands)
-  constexpr int kScaleBytes = 2 * kTile * 4;   // one group's scales: X rows, then W rows
+  constexpr bool kStream = streams(kA);
+  constexpr int kTileM = 64 * kA, kTileN = 64 * kB;
+  constexpr int kSlab = kTileM * kStageK;      // bytes of X's part of a stage
+  constexpr int kStageBytes = (kTileM + kTileN) * kStageK;
+  constexpr int kLoads = kA + kB;              // 16-row loads per wave and stage: kA of X, then kB of W
+  constexpr int kScaleLoads = kTileM / 128;    // 64-row scale loads per wave and group (both operands)
+  constexpr int kScaleBytes = 2 * kTileM * 4;  // one group's scales: X rows, then W rows
+  constexpr int kStores = kB == 3 ? 24 : 32;   // of a wave in an epilogue, at least
   extern __shared__ __attribute__((aligned(16))) char smem[];
   char* scale_smem = smem + kStages * kStageBytes;
   char* bias_smem = scale_smem + kScaleRing * kScaleBytes;
-  [[maybe_unused]] char* turn_smem = bias_smem + kBiasRing * kTile * 4;  // (kStream)
+  [[maybe_unused]] char* turn_smem = bias_smem + kBiasRing * kTileN * 4;  // (kStream)
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wi = wave >> 1, wj = wave & 1;
   const int r = lane & 31, h = lane >> 5;
 
-  Place at = place_of<kTile>(P, blockIdx.x, gridDim.x, 0);  // what is computed; every workgroup has a first task
+  Place at = place_of<kTileM, kTileN>(P, blockIdx.x, gridDim.x, 0);  // what is computed; every workgroup has a first task
   if constexpr (!kStream) {
     const Problem& pr = P.p[at.which];
-    for (int i = threadIdx.x; i < kTile; i += kThreads) {  // read by the epilogue, many barriers from here
+    for (int i = threadIdx.x; i < kTileN; i += kThreads) {  // read by the epilogue, many barriers from here
       float v = 0.f;
       if (pr.bias && at.n0 + i < pr.w.rows)
         v = pr.bias_f32 ? ((const float*)pr.bias)[at.n0 + i] : bf16_to_f32(((const bf16_raw*)pr.bias)[at.n0 + i]);
@@ -201,31 +209,31 @@ __global__ __launch_bounds__(kThreads) void fp8_gemm_kernel(const Problems P) {
   }
 
   // ---- staging: the loads' own cursor, kStages stages ahead of the products and across tiles.
-  // Piece i of a slab = rows (kTile / 4) wave + 16 i .. +15, lane p -> row + p / 4, slot p % 4.
+  // Piece i of a slab = rows (rows / 4) wave + 16 i .. +15, lane p -> row + p / 4, slot p % 4.
   // Rows past the end repeat the last one (never stored).
   // (All offsets fit 32 bits: a tile's rows span at most 256 * 2^22 bytes, a bound the host checks.)
   // Scales: group g = blocks 4 g .. 4 g + 3 of the slice, a dword per row; 64 rows per load, all of one operand:
   // waves 0, 1 fetch the scales of X's rows, waves 2, 3 those of W's.
   __amdgpu_buffer_rsrc_t x_src, w_src, s_src;
-  unsigned x_off[kPieces], w_off[kPieces], s_off[kScaleLoads];
+  unsigned off[kLoads], s_off[kScaleLoads];
   int c_round = 0, c_step = 0, c_steps = 0, c_groups = 0;
   bool c_done = false;
   auto aim = [&](const Place& to) {
     const Operand &X = P.p[to.which].x, &W = P.p[to.which].w;
-    const int x_rows = min(X.rows - to.m0, kTile), w_rows = min(W.rows - to.n0, kTile);
+    const int x_rows = min(X.rows - to.m0, kTileM), w_rows = min(W.rows - to.n0, kTileN);
     const unsigned k_bytes = (unsigned)to.n_steps * kStageK;
     x_src = bounded(X.q + int64_t(to.m0) * X.ld + int64_t(to.first) * kStageK, (unsigned)(x_rows - 1) * (unsigned)X.ld + k_bytes);
     w_src = bounded(W.q + int64_t(to.n0) * W.ld + int64_t(to.first) * kStageK, (unsigned)(w_rows - 1) * (unsigned)W.ld + k_bytes);
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) {
-      const int row = (kTile / 4) * wave + 16 * i + (lane >> 2);
+    for (int i = 0; i < kLoads; ++i) {
+      const bool of_x = i < kA;
+      const int row = of_x ? 16 * kA * wave + 16 * i + (lane >> 2) : 16 * kB * wave + 16 * (i - kA) + (lane >> 2);
       const unsigned chunk = (unsigned)(((lane & 3) ^ ((row >> 2) & 3)) * 16);
-      x_off[i] = (unsigned)min(row, x_rows - 1) * (unsigned)X.ld + chunk;
-      w_off[i] = (unsigned)min(row, w_rows - 1) * (unsigned)W.ld + chunk;
+      off[i] = (unsigned)min(row, (of_x ? x_rows : w_rows) - 1) * (unsigned)(of_x ? X.ld : W.ld) + chunk;
     }
     const Operand& s_op = wave < 2 ? X : W;
     const int s_row0 = wave < 2 ? to.m0 : to.n0, s_last = s_op.rows - 1;
-    const int s_lo = s_row0 >> s_op.shift, s_hi = min(s_row0 + kTile - 1, s_last) >> s_op.shift;
+    const int s_lo = s_row0 >> s_op.shift, s_hi = min(s_row0 + kTileM - 1, s_last) >> s_op.shift;
     s_src = bounded(s_op.scale + int64_t(s_lo) * s_op.ld_scale + to.first / 2,
                     (unsigned)(s_hi - s_lo) * (unsigned)s_op.ld_scale + 4u * (unsigned)((to.n_steps + kGroupStages - 1) / kGroupStages));
 #pragma unroll
@@ -238,10 +246,10 @@ __global__ __launch_bounds__(kThreads) void fp8_gemm_kernel(const Problems P) {
     if constexpr (kStream) {
       // the tile's bias as it lies there, fp32 or pairs of bf16 (whole dwords: 4-byte aligned, a bound the host checks)
       const Problem& pr = P.p[to.which];
-      if (pr.bias && (pr.bias_f32 || wave < 2)) {
+      if (pr.bias && wave * 256 < kTileN * (pr.bias_f32 ? 4 : 2)) {
         const unsigned size = pr.bias_f32 ? 4u : 2u;
         const auto b_src = bounded((const uint8_t*)pr.bias + (unsigned)to.n0 * size, ((unsigned)w_rows * size + 3u) & ~3u);
-        load_to_lds4(b_src, (unsigned)(wave * 64 + lane) * 4u, 0, bias_smem + (c_round & (kBiasRing - 1)) * kTile * 4 + wave * 256);
+        load_to_lds4(b_src, (unsigned)(wave * 64 + lane) * 4u, 0, bias_smem + (c_round & (kBiasRing - 1)) * kTileN * 4 + wave * 256);
       }
     }
   };
@@ -252,7 +260,7 @@ __global__ __launch_bounds__(kThreads) void fp8_gemm_kernel(const Problems P) {
       Place to;
       to.which = -1;
       if constexpr (kStream) {
-        if (!c_done) to = place_of<kTile>(P, blockIdx.x, gridDim.x, ++c_round);
+        if (!c_done) to = place_of<kTileM, kTileN>(P, blockIdx.x, gridDim.x, ++c_round);
       }
       if (to.which < 0) {
         c_done = true;
@@ -271,26 +279,28 @@ __global__ __launch_bounds__(kThreads) void fp8_gemm_kernel(const Problems P) {
   };
   auto issue_one = [&](int slot, int i) {  // i < kLoads
     const unsigned ko = (unsigned)c_step * kStageK;
-    char* dst = smem + slot * kStageBytes + ((kTile / 4) * wave + 16 * (i % kPieces)) * kStageK;
-    if (i < kPieces) load_to_lds16(x_src, x_off[i], ko, dst);
-    else load_to_lds16(w_src, w_off[i - kPieces], ko, dst + kSlab);
+    char* dst = smem + slot * kStageBytes;
+    if (i < kA) load_to_lds16(x_src, off[i], ko, dst + (16 * kA * wave + 16 * i) * kStageK);
+    else load_to_lds16(w_src, off[i], ko, dst + kSlab + (16 * kB * wave + 16 * (i - kA)) * kStageK);
   };
 
-  f32x16 acc[kWB][kWB];
+  f32x16 acc[kA][kB];
 
   // ---- fragment addresses: lane (r, h) reads chunks h and 2 + h of row r of each 32-row block
   const unsigned smem_base = lds_addr(smem);
   const int f = (r >> 2) & 3;
   const unsigned c0 = (unsigned)((h ^ f) << 4), c1 = (unsigned)(((2 + h) ^ f) << 4);
-  const unsigned x_row = (unsigned)((32 * kWB * wi + r) * kStageK);
-  const unsigned w_row = (unsigned)(kSlab + (32 * kWB * wj + r) * kStageK);
-  u32x4 xf[2][kWB][2], wf[2][kWB][2];
-  // read i (0 .. 4 kWB - 1) of the fragments of the stage in `slot`: w0 x0 w1 x1 ..., two chunks each
+  const unsigned x_row = (unsigned)((32 * kA * wi + r) * kStageK);
+  const unsigned w_row = (unsigned)(kSlab + (32 * kB * wj + r) * kStageK);
+  u32x4 xf[2][kA][2], wf[2][kB][2];
+  constexpr int kReads = 2 * (kA + kB);
+  // read i of the fragments of the stage in `slot`: w0 x0 w1 x1 ..., two chunks each, what x has more at the end
   auto frag = [&](int buf, int slot, int i) {
     const unsigned base = smem_base + slot * kStageBytes;
-    const int blk = i >> 2;
-    const unsigned at = base + ((i & 2) ? x_row : w_row) + ((i & 1) ? c1 : c0);
-    u32x4& dst = (i & 2) ? xf[buf][blk][i & 1] : wf[buf][blk][i & 1];
+    const bool of_x = i >= 4 * kB || (i & 2);
+    const int blk = i >= 4 * kB ? kB + (i - 4 * kB) / 2 : i >> 2;
+    const unsigned at = base + (of_x ? x_row : w_row) + ((i & 1) ? c1 : c0);
+    u32x4& dst = of_x ? xf[buf][blk][i & 1] : wf[buf][blk][i & 1];
     if (blk == 0) dst = chunk_read<0>(at);
     if (blk == 1) dst = chunk_read<2048>(at);
     if (blk == 2) dst = chunk_read<4096>(at);
@@ -300,13 +310,14 @@ __global__ __launch_bounds__(kThreads) void fp8_gemm_kernel(const Problems P) {
   auto await_frags = [&](int buf) {
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
-    for (int b = 0; b < kWB; ++b)
-      asm volatile("" : "+v"(xf[buf][b][0]), "+v"(xf[buf][b][1]), "+v"(wf[buf][b][0]), "+v"(wf[buf][b][1]));
+    for (int a = 0; a < kA; ++a) asm volatile("" : "+v"(xf[buf][a][0]), "+v"(xf[buf][a][1]));
+#pragma unroll
+    for (int b = 0; b < kB; ++b) asm volatile("" : "+v"(wf[buf][b][0]), "+v"(wf[buf][b][1]));
   };
-  // scale bytes of the next block (a pair of stages), read 0 .. 2 kWB - 1: X's and W's of each 32-row block in turn
+  // scale bytes of the next block (a pair of stages), read i: X's 32-row blocks, then W's
   const unsigned scale_base = lds_addr(scale_smem);
-  const unsigned xs_row = (unsigned)((32 * kWB * wi + r) * 4), ws_row = (unsigned)((kTile + 32 * kWB * wj + r) * 4);
-  uint32_t xs[kWB], ws[kWB], xs_next[kWB], ws_next[kWB];
+  const unsigned xs_row = (unsigned)((32 * kA * wi + r) * 4), ws_row = (unsigned)((kTileM + 32 * kB * wj + r) * 4);
+  uint32_t xs[kA], ws[kB], xs_next[kA], ws_next[kB];
   unsigned scale_at = scale_base;  // of the block that is read next
   int block = 0, groups = 0;       // its place: block of the tile, group of the workgroup's stream
   auto next_block = [&](bool tile_ends) {
@@ -315,18 +326,24 @@ __global__ __launch_bounds__(kThreads) void fp8_gemm_kernel(const Problems P) {
     scale_at = scale_base + (groups & (kScaleRing - 1)) * kScaleBytes + (block & 3);
   };
   auto read_scale = [&](int i) {
-    const unsigned at = scale_at + ((i & 1) ? ws_row : xs_row);
-    uint32_t& dst = (i & 1) ? ws_next[i >> 1] : xs_next[i >> 1];
-    if ((i >> 1) == 0) asm volatile("ds_read_u8 %0, %1" : "=v"(dst) : "v"(at));
-    if ((i >> 1) == 1) asm volatile("ds_read_u8 %0, %1 offset:128" : "=v"(dst) : "v"(at));
-    if ((i >> 1) == 2) asm volatile("ds_read_u8 %0, %1 offset:256" : "=v"(dst) : "v"(at));
-    if ((i >> 1) == 3) asm volatile("ds_read_u8 %0, %1 offset:384" : "=v"(dst) : "v"(at));
+    const bool of_x = i < kA;
+    const unsigned at = scale_at + (of_x ? xs_row : ws_row);
+    const int blk = of_x ? i : i - kA;
+    uint32_t& dst = of_x ? xs_next[blk] : ws_next[blk];
+    if (blk == 0) asm volatile("ds_read_u8 %0, %1" : "=v"(dst) : "v"(at));
+    if (blk == 1) asm volatile("ds_read_u8 %0, %1 offset:128" : "=v"(dst) : "v"(at));
+    if (blk == 2) asm volatile("ds_read_u8 %0, %1 offset:256" : "=v"(dst) : "v"(at));
+    if (blk == 3) asm volatile("ds_read_u8 %0, %1 offset:384" : "=v"(dst) : "v"(at));
   };
   auto take_scales = [&]() {  // after await_frags
 #pragma unroll
-    for (int b = 0; b < kWB; ++b) {
-      asm volatile("" : "+v"(xs_next[b]), "+v"(ws_next[b]));
-      xs[b] = xs_next[b];
+    for (int a = 0; a < kA; ++a) {
+      asm volatile("" : "+v"(xs_next[a]));
+      xs[a] = xs_next[a];
+    }
+#pragma unroll
+    for (int b = 0; b < kB; ++b) {
+      asm volatile("" : "+v"(ws_next[b]));
       ws[b] = ws_next[b];
     }
   };
@@ -339,14 +356,13 @@ __global__ __launch_bounds__(kThreads) void fp8_gemm_kernel(const Problems P) {
     for (int i = 0; i < kLoads; ++i) issue_one(t, i);
     ++c_step;
   }
-  if constexpr (kWB == 4) asm volatile("s_waitcnt vmcnt(24)" ::: "memory");
-  else asm volatile("s_waitcnt vmcnt(12)" ::: "memory");
+  wait_vm<3 * kLoads>();
   __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-  for (int i = 0; i < 2 * kWB; ++i) read_scale(i);
+  for (int i = 0; i < kA + kB; ++i) read_scale(i);
 #pragma unroll
-  for (int i = 0; i < 4 * kWB; ++i) frag(0, 0, i);
+  for (int i = 0; i < kReads; ++i) frag(0, 0, i);
   await_frags(0);
   take_scales();
 
@@ -354,9 +370,9 @@ __global__ __launch_bounds__(kThreads) void fp8_gemm_kernel(const Problems P) {
   int fresh = 0;  // stages since an epilogue left its stores in flight: see below
   for (int round = 0;;) {
 #pragma unroll
-    for (int a = 0; a < kWB; ++a)
+    for (int a = 0; a < kA; ++a)
 #pragma unroll
-      for (int b = 0; b < kWB; ++b)
+      for (int b = 0; b < kB; ++b)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[a][b][e] = 0.f;
 
@@ -367,25 +383,25 @@ __global__ __launch_bounds__(kThreads) void fp8_gemm_kernel(const Problems P) {
         // Stage t + u + 1 has landed: two younger stages may be in flight (anything else among them makes the count
         // strict by that much), and in the first three stages after an epilogue its stores too, which lie between
         // that stage and the youngest. After the barrier everyone's part has, and nobody reads this slot any more.
-        if constexpr (kWB == 4) {
+        if constexpr (kStream) {
           // (the branch is inside the block: around a branch of its own the compiler would sink products)
-          asm volatile("s_cmp_gt_i32 %0, 0\n\ts_cbranch_scc1 .Lfresh%=\n\ts_waitcnt vmcnt(16)\n.Lfresh%=:\n\ts_waitcnt vmcnt(48)"
-                       ::"s"(fresh)
+          asm volatile("s_cmp_gt_i32 %0, 0\n\ts_cbranch_scc1 .Lfresh%=\n\ts_waitcnt vmcnt(%1)\n.Lfresh%=:\n\ts_waitcnt vmcnt(%2)"
+                       ::"s"(__builtin_amdgcn_readfirstlane(fresh)), "i"(2 * kLoads), "i"(2 * kLoads + kStores)
                        : "memory", "scc");
           fresh = max(fresh - 1, 0);
         } else {
-          asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+          wait_vm<2 * kLoads>();
         }
         __builtin_amdgcn_s_barrier();
         if (u == 0) turn();
         __builtin_amdgcn_sched_barrier(0);
         const int next = (slot + 1) & (kStages - 1);
-        constexpr int kProducts = kWB * kWB;
+        constexpr int kProducts = kA * kB;
         int reads = 0, loads = 0, scales = 0;
-        [[maybe_unused]] bf16x8 xb[4], wb[kWide ? kWB : 1][4];
+        [[maybe_unused]] bf16x8 xb[4], wb[kWide ? kB : 1][4];
 #pragma unroll
         for (int i = 0; i < kProducts; ++i) {
-          const int a = i / kWB, b = i % kWB;
+          const int a = i / kB, b = i % kB;
           if constexpr (kWide) {
             if (b == 0) {
 #pragma unroll
@@ -401,10 +417,10 @@ __global__ __launch_bounds__(kThreads) void fp8_gemm_kernel(const Problems P) {
             acc[a][b] = mfma_scaled(join(wf[u][b][0], wf[u][b][1]), join(xf[u][a][0], xf[u][a][1]), acc[a][b], ws[b], xs[a]);
           }
 #pragma unroll
-          for (; reads < (i + 1) * 4 * kWB / kProducts; ++reads) frag(u ^ 1, next, reads);
+          for (; reads < (i + 1) * kReads / kProducts; ++reads) frag(u ^ 1, next, reads);
           if (u == 1) {
 #pragma unroll
-            for (; scales < (i + 1) * 2 * kWB / kProducts; ++scales) read_scale(scales);
+            for (; scales < (i + 1) * (kA + kB) / kProducts; ++scales) read_scale(scales);
           }
 #pragma unroll
           for (; loads < (i + 1) * kLoads / kProducts; ++loads) issue_one(slot, loads);
@@ -418,7 +434,7 @@ __global__ __launch_bounds__(kThreads) void fp8_gemm_kernel(const Problems P) {
       take_scales();
     }
 
-    // ---- epilogue: register e of acc[a][b]: token m0 + 32 kWB wi + 32 a + r, feature n0 + 32 kWB wj + 32 b +
+    // ---- epilogue: register e of acc[a][b]: token m0 + 32 kA wi + 32 a + r, feature n0 + 32 kB wj + 32 b +
     // 8 (e / 4) + 4 h + (e & 3). Through LDS, so that rows leave in whole lines: staged row = token, its 16-byte
     // chunks XOR-permuted with the token, so the lanes of a write (32 tokens, one feature offset) and of a read
     // (whole tokens) both spread over the banks.
@@ -428,12 +444,12 @@ __global__ __launch_bounds__(kThreads) void fp8_gemm_kernel(const Problems P) {
     const int64_t slice0 = int64_t(at.slice) * M * N;
     if constexpr (kStream) {
       // The next tile's loads are on their way and its first fragments in registers: a wave turns its quarter around
-      // in 4 KiB of its own, 32 tokens x 128 bytes at a time, meets nobody, and goes on without waiting for its
+      // in LDS of its own, 32 tokens x 128 (kB = 3: 192) bytes at a time, meets nobody, and goes on without waiting for its
       // stores. LDS by inline assembly (in order within a wave): the compiler would wait for the loads in flight.
 #pragma unroll
-      for (int a = 0; a < kWB; ++a)
+      for (int a = 0; a < kA; ++a)
 #pragma unroll
-        for (int b = 0; b < kWB; ++b) asm volatile("" : "+a"(acc[a][b]));
+        for (int b = 0; b < kB; ++b) asm volatile("" : "+a"(acc[a][b]));
       int el = lane;
       asm volatile("" : "+v"(el));  // (addresses are formed here, not held through the products)
       const int er = el & 31, eh = el >> 5;
@@ -441,44 +457,54 @@ __global__ __launch_bounds__(kThreads) void fp8_gemm_kernel(const Problems P) {
       const int has_bias = __builtin_amdgcn_readfirstlane(pr.bias != nullptr);  // (held: not fetched after every store)
       auto store_quarter = [&](auto out_f32) {
         using Out = std::conditional_t<decltype(out_f32)::value, float, bf16_raw>;
-        constexpr int kSize = (int)sizeof(Out), kVec = 16 / kSize, kB = 4 / kSize;  // kB: feature blocks turned together
+        constexpr int kSize = (int)sizeof(Out), kVec = 16 / kSize;
+        constexpr int kT = kSize == 4 ? 1 : kB == 3 ? 3 : 2;                  // feature blocks turned together
+        constexpr int kRow = 32 * kT * kSize, kChunks = kRow / 16;            // bytes and chunks of a token
+        constexpr int kMoves = 32 * kChunks / 64, kSwap = kChunks == 8 ? 7 : 3;  // chunks XORed with the token's low bits
         Out* out = (Out*)pr.out + slice0 + int64_t(m0) * N;
-        const auto dst = __builtin_amdgcn_make_buffer_rsrc((void*)out, 0, (int)((unsigned)min(M - m0, kTile) * (unsigned)N * kSize), 0x00027000);
-        const unsigned turn_base = lds_addr(turn_smem) + wave * kWaveStage;
-        const unsigned bias_base = lds_addr(bias_smem) + (round & (kBiasRing - 1)) * kTile * 4;
+        const auto dst = __builtin_amdgcn_make_buffer_rsrc((void*)out, 0, (int)((unsigned)min(M - m0, kTileM) * (unsigned)N * kSize), 0x00027000);
+        const unsigned turn_base = lds_addr(turn_smem) + wave * wave_turn_bytes(kB);
+        const unsigned bias_base = lds_addr(bias_smem) + (round & (kBiasRing - 1)) * kTileN * 4;
 #pragma unroll
-        for (int b0 = 0; b0 < kWB; b0 += kB) {
-          f32x4 bv[kB][4];
+        for (int b0 = 0; b0 < kB; b0 += kT) {
+          f32x4 bv[kT][4];
 #pragma unroll
-          for (int i = 0; i < 4 * kB; ++i) bv[i / 4][i % 4] = f32x4{0.f, 0.f, 0.f, 0.f};
-          const unsigned b_col = (unsigned)(32 * (kWB * wj + b0) + 4 * eh);
+          for (int i = 0; i < 4 * kT; ++i) bv[i / 4][i % 4] = f32x4{0.f, 0.f, 0.f, 0.f};
+          const unsigned b_col = (unsigned)(32 * (kB * wj + b0) + 4 * eh);
           if (has_bias && bias_f32) {
 #pragma unroll
-            for (int i = 0; i < 4 * kB; ++i) asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(bv[i / 4][i % 4]) : "v"(bias_base + b_col * 4), "i"(32 * i));
+            for (int i = 0; i < 4 * kT; ++i) asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(bv[i / 4][i % 4]) : "v"(bias_base + b_col * 4), "i"(32 * i));
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
-            for (int i = 0; i < 4 * kB; ++i) asm volatile("" : "+v"(bv[i / 4][i % 4]));
+            for (int i = 0; i < 4 * kT; ++i) asm volatile("" : "+v"(bv[i / 4][i % 4]));
           } else if (has_bias) {
-            u32x2 w[4 * kB];
+            u32x2 w[4 * kT];
 #pragma unroll
-            for (int i = 0; i < 4 * kB; ++i) asm volatile("ds_read_b64 %0, %1 offset:%2" : "=v"(w[i]) : "v"(bias_base + b_col * 2), "i"(16 * i));
+            for (int i = 0; i < 4 * kT; ++i) asm volatile("ds_read_b64 %0, %1 offset:%2" : "=v"(w[i]) : "v"(bias_base + b_col * 2), "i"(16 * i));
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 #pragma unroll
-            for (int i = 0; i < 4 * kB; ++i) {
+            for (int i = 0; i < 4 * kT; ++i) {
               asm volatile("" : "+v"(w[i]));
               bv[i / 4][i % 4] = f32x4{__uint_as_float(w[i][0] << 16), __uint_as_float(w[i][0] & 0xffff0000u),
                                        __uint_as_float(w[i][1] << 16), __uint_as_float(w[i][1] & 0xffff0000u)};
             }
           }
-          const int col = n0 + 32 * (kWB * wj + b0) + (el & 7) * kVec;
-          const unsigned row0 = (unsigned)(32 * kWB * wi + (el >> 3)) * (unsigned)N * kSize;
-          const unsigned at0 = col + kVec <= N ? row0 + (unsigned)col * kSize : 0x80000000u;
-          const bool ragged = N % kVec != 0 && n0 + 32 * (kWB * wj + b0 + kB) > N;
+          // lane l moves chunk (64 i + l) % kChunks of token (64 i + l) / kChunks
+          unsigned from[kMoves], to_at[kMoves];
+          int to_col[kMoves];
+#pragma unroll
+          for (int i = 0; i < kMoves; ++i) {
+            const int token = (64 * i + el) / kChunks, chunk = (64 * i + el) % kChunks;
+            from[i] = turn_base + token * kRow + ((chunk ^ (token & kSwap)) << 4);
+            to_col[i] = n0 + 32 * (kB * wj + b0) + chunk * kVec;
+            to_at[i] = ((unsigned)(32 * kA * wi + token) * (unsigned)N + (unsigned)to_col[i]) * kSize;
+          }
+          const bool ragged = N % kVec != 0 && n0 + 32 * (kB * wj + b0 + kT) > N;
           using Piece = std::conditional_t<kSize == 2, u32x2, f32x4>;  // four features of a token
-          Piece piece[kB][4];
+          Piece piece[kT][4];
           auto round_up = [&](int a) {  // one block at a time leaves the accumulator file
 #pragma unroll
-            for (int b = 0; b < kB; ++b) {
+            for (int b = 0; b < kT; ++b) {
               f32x16 v = acc[a][b0 + b];
               asm volatile("" : "+v"(v));
 #pragma unroll
@@ -491,34 +517,34 @@ __global__ __launch_bounds__(kThreads) void fp8_gemm_kernel(const Problems P) {
           };
           round_up(0);
 #pragma unroll
-          for (int a = 0; a < kWB; ++a) {
+          for (int a = 0; a < kA; ++a) {
 #pragma unroll
-            for (int b = 0; b < kB; ++b)
+            for (int b = 0; b < kT; ++b)
 #pragma unroll
               for (int g = 0; g < 4; ++g) {
                 const unsigned chunk = (unsigned)(32 * b + 8 * g + 4 * eh) / kVec;
-                const unsigned to = turn_base + er * 128 + ((chunk ^ (er & 7)) << 4) + (kSize == 2 ? 8 * eh : 0);
+                const unsigned to = turn_base + er * kRow + ((chunk ^ (er & kSwap)) << 4) + (kSize == 2 ? 8 * eh : 0);
                 if constexpr (kSize == 2) asm volatile("ds_write_b64 %0, %1" ::"v"(to), "v"(piece[b][g]) : "memory");
                 else asm volatile("ds_write_b128 %0, %1" ::"v"(to), "v"(piece[b][g]) : "memory");
               }
-            u32x4 w[4];
-            const unsigned from = turn_base + (el >> 3) * 128 + (((el & 7) ^ (el >> 3)) << 4);
-            w[0] = chunk_read<0>(from);
-            w[1] = chunk_read<1024>(from);
-            w[2] = chunk_read<2048>(from);
-            w[3] = chunk_read<3072>(from);
-            if (a + 1 < kWB) round_up(a + 1);  // while they come
-            asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3])::"memory");
-            // Rows at any alignment. Out of range (rows past M, pieces past or across N): dropped, but issued and counted.
+            u32x4 w[kMoves];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              __builtin_amdgcn_raw_buffer_store_b128(w[i], dst, (int)(at0 + (unsigned)((32 * a + 8 * i) * N) * kSize), 0, 0);
+            for (int i = 0; i < kMoves; ++i) w[i] = chunk_read<0>(from[i]);
+            if (a + 1 < kA) round_up(a + 1);  // while they come
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+            for (int i = 0; i < kMoves; ++i) asm volatile("" : "+v"(w[i]));
+            // Rows at any alignment. Out of range (rows past M, pieces past or across N): dropped, but issued and counted.
+            const unsigned down = (unsigned)(32 * a * N) * kSize;
+#pragma unroll
+            for (int i = 0; i < kMoves; ++i)
+              __builtin_amdgcn_raw_buffer_store_b128(w[i], dst, (int)(to_col[i] + kVec <= N ? to_at[i] + down : 0x80000000u), 0, 0);
             if (ragged) {  // wave-uniform: the piece across N, one element at a time
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
+              for (int i = 0; i < kMoves; ++i)
 #pragma unroll
                 for (int e = 0; e + 1 < kVec; ++e) {
-                  const unsigned to = col + kVec > N && col + e < N ? row0 + (unsigned)((32 * a + 8 * i) * N + col + e) * kSize : 0x80000000u;
+                  const unsigned to = to_col[i] + kVec > N && to_col[i] + e < N ? to_at[i] + down + e * kSize : 0x80000000u;
                   if constexpr (kSize == 4) __builtin_amdgcn_raw_buffer_store_b32(w[i][e], dst, (int)to, 0, 0);
                   else __builtin_amdgcn_raw_buffer_store_b16((unsigned short)(w[i][e / 2] >> (16 * (e & 1))), dst, (int)to, 0, 0);
                 }
@@ -527,30 +553,30 @@ __global__ __launch_bounds__(kThreads) void fp8_gemm_kernel(const Problems P) {
           }
         }
       };
-      // (at least 32 stores of a wave: the count of the three stages that follow)
+      // (at least kStores stores of a wave: the count of the three stages that follow)
       if (pr.out_f32) store_quarter(std::true_type{});
       else store_quarter(std::false_type{});
       fresh = 3;
-      at = place_of<kTile>(P, blockIdx.x, gridDim.x, ++round);
+      at = place_of<kTileM, kTileN>(P, blockIdx.x, gridDim.x, ++round);
       if (at.which < 0) break;
     } else {
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the tail's unused loads have left LDS alone
       __syncthreads();                                  // and nobody reads the ring any more: it stages the output
       auto store_tile = [&](auto out_f32) {
         using Out = std::conditional_t<decltype(out_f32)::value, float, bf16_raw>;
-        constexpr int kRowBytes = kTile * (int)sizeof(Out), kVec = 16 / (int)sizeof(Out);
+        constexpr int kRowBytes = kTileN * (int)sizeof(Out), kVec = 16 / (int)sizeof(Out);
         constexpr int kChunks = kRowBytes / 16;
         Out* out = (Out*)pr.out + slice0;
 #pragma unroll
-        for (int a = 0; a < kWB; ++a)
+        for (int a = 0; a < kA; ++a)
 #pragma unroll
-          for (int b = 0; b < kWB; ++b) {
+          for (int b = 0; b < kB; ++b) {
             f32x16 v = acc[a][b];
             asm volatile("" : "+v"(v));  // one block at a time leaves the accumulator file
-            const int row = 32 * (kWB * wi + a) + r;
+            const int row = 32 * (kA * wi + a) + r;
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-              const int col = 32 * (kWB * wj + b) + 8 * g + 4 * h;
+              const int col = 32 * (kB * wj + b) + 8 * g + 4 * h;
               const f32x4 bv = *reinterpret_cast<const f32x4*>(bias_smem + col * 4);
               const int to = row * kRowBytes + (((col / kVec) ^ (r & (kChunks - 1))) * 16) + (col % kVec) * (int)sizeof(Out);
               if constexpr (sizeof(Out) == 2)
@@ -564,7 +590,7 @@ __global__ __launch_bounds__(kThreads) void fp8_gemm_kernel(const Problems P) {
         const int ch = threadIdx.x % kChunks, n = n0 + ch * kVec;
         if (n < N) {
 #pragma unroll 4
-          for (int q = threadIdx.x / kChunks; q < kTile; q += kThreads / kChunks) {
+          for (int q = threadIdx.x / kChunks; q < kTileM; q += kThreads / kChunks) {
             const u32x4 w = *reinterpret_cast<const u32x4*>(smem + q * kRowBytes + ((ch ^ (q & 31 & (kChunks - 1))) * 16));
             if (m0 + q >= M) break;
             Out* to = out + int64_t(m0 + q) * N + n;
@@ -656,13 +682,13 @@ __global__ __launch_bounds__(kThreads) void fold_kernel(const Folds folds) {
   }
 }
 
-template <int kWB, bool kWide>
+template <int kA, int kB, bool kWide>
 void launch(const Problems& P, hipStream_t stream) {
-  constexpr int kLds = lds_bytes(kWB);
-  (void)hipFuncSetAttribute((const void*)fp8_gemm_kernel<kWB, kWide>, hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+  constexpr int kLds = lds_bytes(kA, kB);
+  (void)hipFuncSetAttribute((const void*)fp8_gemm_kernel<kA, kB, kWide>, hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
   const int tasks = P.p[0].tasks + P.p[1].tasks;
-  const unsigned blocks = (unsigned)(kWB == 4 ? std::min(tasks, kSlots) : tasks);
-  hipLaunchKernelGGL((fp8_gemm_kernel<kWB, kWide>), dim3(blocks), dim3(kThreads), kLds, stream, P);
+  const unsigned blocks = (unsigned)(streams(kA) ? std::min(tasks, kSlots) : tasks);
+  hipLaunchKernelGGL((fp8_gemm_kernel<kA, kB, kWide>), dim3(blocks), dim3(kThreads), kLds, stream, P);
 }
 
 }  // namespace
@@ -670,12 +696,13 @@ void launch(const Problems& P, hipStream_t stream) {
 // Which tile, and how many slices of the contraction: the smallest estimated time, in microseconds fitted to
 // measurements of 14 shapes from 16 x 3840 x 1280 to 8192 x 22016 x 4096 (most within 10 %).
 // 256 tile: workgroups stream through their tasks, dealt as place_of does; a stage takes 0.75 with every compute
-// unit busy (0.47 alone), a tile 3 more (its epilogue), the launch 10 (first loads, last stores).
+// unit busy (0.47 alone), a tile 3 more (its epilogue), the launch 10 (first loads, last stores). The 192 tile takes
+// 0.61 (0.37) a stage: dearer per product, but it fills a round that 256 leaves half empty.
 // 128 tile: rounds of workgroups over two slots a compute unit; a stage takes 0.20 alone, 0.29 with one workgroup
 // per compute unit, 0.60 with two, a workgroup 3.3 more. The widened products have this tile only, at 1.5 times
 // its stage.
-// So 8192 x 1280 x 5120 takes the 256 tile (160 of them: 63 against 77), 2048^3 the 128 tile (13 against 28), and
-// the two gradients of 8192 x 1280 -> 5120 together the 256 tile (260 of two lengths: 128 against 162).
+// So 8192 x 1280 x 5120 takes the 192 tile (224 of them: 57; 160 of 256: 62; 128: 77), 2048^3 the 128 tile (13
+// against 28), and the two gradients of 8192 x 1280 -> 5120 together a large tile (128 against 162).
 // A slice's partial sums are written and read again at some 4.5 TB/s and folded by a launch of 3: 1024 x 1024 x
 // 8192 gains by four slices (33 -> 23), 2048^3 loses by two (13 -> 31).
 struct Work {
@@ -683,9 +710,10 @@ struct Work {
   int steps;
 };
 
-static float time_256(const Work* work, int n) {  // the longer tasks first
+static float time_stream(int tile, const Work* work, int n) {  // the longer tasks first
   const int64_t first = work[0].tasks, total = first + (n > 1 ? work[1].tasks : 0);
-  const float stage = 0.47f + 0.28f * (total < kSlots ? total / float(kSlots) : 1.f);
+  const float load = total < kSlots ? total / float(kSlots) : 1.f;
+  const float stage = tile == 256 ? 0.47f + 0.28f * load : 0.37f + 0.24f * load;
   auto task = [&](int64_t i) { return i >= total ? 0.f : 3.f + stage * work[i >= first].steps; };
   const int64_t rounds = ceil_div(total, kSlots);
   if (n == 1) return 10.f + rounds * task(0);
@@ -722,8 +750,11 @@ struct Choice {
   float time;
 };
 
+// A tile is named by its features: 256 (and 256 tokens), 192 (256 tokens) or 128 (128 tokens).
+static int64_t tiles_of(int tile, int M, int N) { return ceil_div(M, tile == 128 ? 128 : 256) * ceil_div(N, tile); }
+
 static Work work_of(const Fp8GemmPlan& plan, const Fp8GemmProblem& p) {
-  return Work{ceil_div(p.x.rows, plan.tile) * ceil_div(p.w.rows, plan.tile) * plan.slices, std::min(plan.steps_per_slice, p.K / kStageK)};
+  return Work{tiles_of(plan.tile, p.x.rows, p.w.rows) * plan.slices, std::min(plan.steps_per_slice, p.K / kStageK)};
 }
 static float fold_time(const Fp8GemmPlan& plan, const Fp8GemmProblem& p) {
   return plan.slices == 1 ? 0.f : 3.f + float(p.x.rows) * p.w.rows * (8.f * plan.slices + 2.f) / 4.5e6f;
@@ -737,7 +768,7 @@ static float time_of(const Fp8GemmPlan* plans, const Fp8GemmProblem* problems, i
     t += fold_time(plans[i], problems[i]);
   }
   if (n == 2 && work[1].steps > work[0].steps) std::swap(work[0], work[1]);
-  return t + (plans[0].tile == 256 ? time_256(work, n) : time_128(work, n, problems[0].out_dtype == kF32));
+  return t + (plans[0].tile != 128 ? time_stream(plans[0].tile, work, n) : time_128(work, n, problems[0].out_dtype == kF32));
 }
 
 static Choice choose(int tile, const Fp8GemmProblem* problems, int n) {
@@ -765,15 +796,17 @@ static Choice choose(int tile, const Fp8GemmProblem* problems, int n) {
 }
 
 void fp8_gemm_plan(Fp8GemmProblem* problems, int n) {
-  bool small = false;  // no 256 tile: widened products, or what its epilogue's 32-bit offsets and bias loads do not reach
+  bool small = false;  // no large tile: widened products, or what its epilogue's 32-bit offsets and bias loads do not reach
   for (int i = 0; i < n; ++i) {
     const Fp8GemmProblem& p = problems[i];
     small |= p.out_dtype == kF32 || p.w.rows > (1 << 20) || reinterpret_cast<uintptr_t>(p.bias) % 4 != 0;
   }
   Choice best = choose(128, problems, n);
   if (!small) {
-    const Choice big = choose(256, problems, n);
-    if (big.time < best.time) best = big;
+    for (int tile : {192, 256}) {
+      const Choice big = choose(tile, problems, n);
+      if (big.time < best.time) best = big;
+    }
   }
   for (int i = 0; i < n; ++i) problems[i].plan = best.plan[i];
 }
@@ -795,7 +828,7 @@ void fp8_gemm(const Fp8GemmProblem* problems, int n, const Fp8ColumnSums* sums, 
     const bool fold = g.partial != nullptr;
     const bool f32 = fold || g.out_dtype == kF32;
     void* out = fold ? (void*)g.partial : g.out;
-    const int64_t tasks = ceil_div(M, g.plan.tile) * ceil_div(N, g.plan.tile) * g.plan.slices;
+    const int64_t tasks = tiles_of(g.plan.tile, M, N) * g.plan.slices;
     ps[i] = Problem{operand(g.x), operand(g.w), out, fold ? nullptr : g.bias, f32, g.bias_dtype == kF32,
                     g.K / kStageK, g.plan.steps_per_slice, (int)tasks};
     if (fold)
@@ -804,9 +837,10 @@ void fp8_gemm(const Fp8GemmProblem* problems, int n, const Fp8ColumnSums* sums, 
   }
   auto go = [&](const Problem& a, const Problem* b, int tile, bool wide) {
     Problems P = {{a, b ? *b : Problem{}}};
-    if (wide) launch<2, true>(P, stream);
-    else if (tile == 256) launch<4, false>(P, stream);
-    else launch<2, false>(P, stream);
+    if (wide) launch<2, 2, true>(P, stream);
+    else if (tile == 256) launch<4, 4, false>(P, stream);
+    else if (tile == 192) launch<4, 3, false>(P, stream);
+    else launch<2, 2, false>(P, stream);
   };
   auto wide = [&](int i) { return problems[i].out_dtype == kF32; };
   if (n == 2 && problems[0].plan.tile == problems[1].plan.tile && wide(0) == wide(1)) {

@@ -111,7 +111,8 @@ def test_product(m, n, k, dtype, tiles):
         check_product(b, a, None, dtype, ops.fp8_matmul(b, a, None, dtype))  # tiles on the left
 
 
-@pytest.mark.parametrize("m,n,k", [(8192, 5120, 1280), (8100, 5001, 1300), (16500, 2600, 1400), (2000, 2048, 65536), (2000, 2001, 65536)])
+@pytest.mark.parametrize("m,n,k", [(8192, 5120, 1280), (8100, 5001, 1300), (16500, 2600, 1400), (2000, 2048, 65536), (2000, 2001, 65536),
+                                   (8192, 1280, 5120), (16384, 1403, 1300), (2000, 1501, 65536)])
 @pytest.mark.parametrize("bias", [None, torch.bfloat16, torch.float32])
 def test_product_of_many_tiles(m, n, k, bias):
     """Sizes at which a workgroup goes through several tiles, and through slices of a long contraction."""
