@@ -7,8 +7,8 @@
 // vector instruction per product more than an unscaled one.
 //
 // Structure. A workgroup of 4 waves (2 x 2) owns an output tile of 128 x 128, 256 x 192 or 256 x 256 (tokens x
-// features), each wave a quarter as kA x kB blocks of 32 x 32. A pipeline stage is 64 values of the contraction: [tile rows][64 bytes] of each
-// operand, moved global -> LDS by buffer loads into a ring of four. The body of stage t
+// features), each wave a quarter as kA x kB blocks of 32 x 32. A pipeline stage is 64 values of the contraction:
+// [tile rows][64 bytes] of each operand, moved global -> LDS by buffer loads into a ring of four. The body of stage t
 //   * waits until stage t + 1 has landed (counted: two younger stages stay in flight) and meets the
 //     other waves, who by then have read stage t out of LDS;
 //   * issues the products of stage t from registers, and between them the LDS reads of stage t + 1 and
