@@ -28,7 +28,7 @@ __device__ __forceinline__ unsigned lds_addr(const char* p) {
 }
 
 // ---- LDS reads in flight. An asm output counts as written at once, so nothing may touch it before wait_for
-// (which ties the registers to the wait). kYounger: reads requested after the one awaited.
+// (which ties the registers to the wait): a kernel that uses these must not spill, its register budget is chosen so. kYounger: reads requested after the one awaited.
 template <int kOff>
 __device__ __forceinline__ u32x4 read16(unsigned addr) {
   u32x4 v;
@@ -194,9 +194,37 @@ __device__ __forceinline__ bool visible(const Shape& s, int q, int key) {
   return key <= q && (q - key < s.window || key < s.sinks);
 }
 
+// A wave's 32 rows of results, turned around in LDS of its own so that they leave in whole rows (from the
+// accumulators a store would touch 32 rows with 16 bytes each). The 16-byte chunks of a row are XORed with its index.
+template <int D, int kSize>  // kSize: bytes of a value, 2 or 1
+struct RowTurn {
+  static constexpr int kRow = D * kSize, kChunks = kRow / 16, kBytes = 32 * kRow;
+  __device__ __forceinline__ static char* at(char* mem, int row, int chunk) {
+    return mem + row * kRow + ((chunk ^ (row & (kChunks - 1))) << 4);
+  }
+  // columns 32 db + 8 g + 4 h .. +3 of row r
+  template <typename V>
+  __device__ __forceinline__ static void put(char* mem, int r, int h, int db, int g, V w) {
+    static_assert(sizeof(V) == 4 * kSize);
+    const int byte = (32 * db + 8 * g) * kSize;
+    *reinterpret_cast<V*>(at(mem, r, byte / 16) + byte % 16 + 4 * h * kSize) = w;
+  }
+  // the first `rows` rows to `to`, `pitch` bytes apart
+  __device__ __forceinline__ static void store(const char* mem, char* to, int64_t pitch, int rows, int lane) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own writes
+#pragma unroll
+    for (int i = 0; i < kBytes / 1024; ++i) {
+      const int row = (64 * i + lane) / kChunks, chunk = (64 * i + lane) % kChunks;
+      const u32x4 w = *reinterpret_cast<const u32x4*>(at(const_cast<char*>(mem), row, chunk));
+      if (row < rows) *reinterpret_cast<u32x4*>(to + row * pitch + chunk * 16) = w;
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // before it is written again
+  }
+};
+
 // Score accumulators of the 32 keys from `key0` on start from minus infinity where the query (on the lane) does
 // not see the key: the products leave it there, so the maximum ignores it and its probability is zero.
-__device__ __forceinline__ void start_masked(const Shape& s, int q_row, int key0, int h, f32x16& acc) {
+__device__ __forceinline__ void start_masked(const Shape& s, int q_row, int key0, int h, float (&acc)[16]) {
   __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
   for (int i = 0; i < 16; ++i) {

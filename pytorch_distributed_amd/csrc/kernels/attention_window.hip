@@ -22,9 +22,10 @@
 // each of them. Each read is requested kAhead products before the one that takes it and awaited by count.
 //
 // What bounds them: latency, hidden by as many waves as the registers allow. 1 x 8192, 32 heads of 128, window 1024,
-// 4 sinks: forward 210 us (matrix pipes 31 % busy, two waves on a SIMD), dQ 261 (38 %; at one wave 361), dK / dV 349
-// and 43 for the far sinks. 8 x 1024, 20 heads of 64, window 256, forward: 33 us (four waves; at three 40), there the
-// vector unit's exponentials weigh as much as the products.
+// 4 sinks: forward 201 us (matrix pipes 31 % busy, two waves on a SIMD), dQ 262 (38 %; at one wave 361), dK / dV 350
+// and 44 for the far sinks. 8 x 1024, 20 heads of 64, window 256: forward 33 us (four waves; at three 40; 37 with the
+// rest for the backward), dQ 47, dK / dV 42 (three waves each); there the vector unit's exponentials weigh as much
+// as the products. Results leave through LDS in whole rows (dK / dV 48 -> 43 there).
 //
 // Every sum has one owner and a fixed order: results repeat bit for bit. Probabilities and their gradients
 // are rounded to bf16 as operands of the second products (relative 2^-9 each, averaged by the sums); scores,
@@ -127,14 +128,15 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
       constexpr int kN = 2 * kKSteps;
       static_for<0, kAhead>(request);
       f32x16 s_acc[2];
+      float first[2][16] = {};
+      if (tile_masked(s, key0, q0)) {  // wave-uniform
+        start_masked(s, q_row, key0, h, first[0]);
+        start_masked(s, q_row, key0 + 32, h, first[1]);
+      }
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s_acc[kb][i] = 0.f;
-      if (tile_masked(s, key0, q0)) {  // wave-uniform
-        start_masked(s, q_row, key0, h, s_acc[0]);
-        start_masked(s, q_row, key0 + 32, h, s_acc[1]);
-      }
+        for (int i = 0; i < 16; ++i) s_acc[kb][i] = first[kb][i];
       static_for<0, kN>([&](auto n) {
         constexpr int kb = n % 2, ks = n / 2;
         wait_for<(kN - 1 - n < kAhead - 1 ? kN - 1 - n : kAhead - 1)>(kf[n % kAhead]);
@@ -223,26 +225,31 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load to LDS outlives the workgroup
 
+  __syncthreads();  // nobody reads the tiles any more
+  if (!wave_active) return;
   const float l_tot = lane_pair_sum(l_run);
-  if (q_row < T) {
-    const float inv_l = 1.f / l_tot;
-    const int64_t row = (int64_t(b) * T + q_row) * (int64_t(s.H) * D) + int64_t(head) * D;
+  const float inv_l = 1.f / l_tot;
+  using Out = RowTurn<D, 2>;
+  using Rest = RowTurn<D, 1>;
+  char* mine = smem + wave * (Out::kBytes + Rest::kBytes);
 #pragma unroll
-    for (int db = 0; db < kDBlocks; ++db)
+  for (int db = 0; db < kDBlocks; ++db)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        float o[4];
+    for (int g = 0; g < 4; ++g) {
+      float o[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = o_acc[db][4 * g + e] * inv_l;
-        const u32x2 w = {pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
-        *reinterpret_cast<u32x2*>(out + row + db * 32 + 8 * g + 4 * h) = w;
-        if (out_rest)
-          *reinterpret_cast<uint32_t*>(out_rest + row + db * 32 + 8 * g + 4 * h) =
-              pack_rest(o[0] - bf16_lo(w[0]), o[1] - bf16_hi(w[0]), o[2] - bf16_lo(w[1]), o[3] - bf16_hi(w[1]));
-      }
-    // minus the row's log-sum of exponentials, in units of a score: what the backward's S chains start from
-    if (h == 0) neg_lse_out[int64_t(bh) * T + q_row] = -(m_run + __log2f(l_tot)) / c;
-  }
+      for (int e = 0; e < 4; ++e) o[e] = o_acc[db][4 * g + e] * inv_l;
+      const u32x2 w = {pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3])};
+      Out::put(mine, r, h, db, g, w);
+      if (out_rest)
+        Rest::put(mine + Out::kBytes, r, h, db, g,
+                  pack_rest(o[0] - bf16_lo(w[0]), o[1] - bf16_hi(w[0]), o[2] - bf16_lo(w[1]), o[3] - bf16_hi(w[1])));
+    }
+  const int64_t row = (int64_t(b) * T + q0) * (int64_t(s.H) * D) + int64_t(head) * D;
+  Out::store(mine, reinterpret_cast<char*>(out + row), int64_t(s.H) * D * 2, T - q0, lane);
+  if (out_rest) Rest::store(mine + Out::kBytes, reinterpret_cast<char*>(out_rest + row), int64_t(s.H) * D, T - q0, lane);
+  // minus the row's log-sum of exponentials, in units of a score: what the backward's S chains start from
+  if (h == 0 && q_row < T) neg_lse_out[int64_t(bh) * T + q_row] = -(m_run + __log2f(l_tot)) / c;
 }
 
 // ============================================================================ dQ
@@ -258,7 +265,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
   constexpr int kKSteps = D / 16;
   constexpr int kDBlocks = D / 32;
   constexpr int kTileBytes = kBN * D * 2;
-  constexpr int kAhead = 6;  // fragments in flight
+  constexpr int kAhead = D == 128 && kDrop ? 3 : 6;  // fragments in flight (the dropout words take registers)
   extern __shared__ __attribute__((aligned(256))) char smem[];
 
   const int lane = threadIdx.x & 63;
@@ -345,14 +352,16 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
       f32x16 s_acc, dp_acc;  // of the half in hand
       bf16x8 ds[4];
       auto start = [&](int kb) {
-        float s0 = neg_lse, dp0 = -delta;
+        float s0 = neg_lse, dp0 = -delta, first[16];
         asm volatile("" : "+v"(s0), "+v"(dp0));  // (16 copies each are made here, not held through the loop)
 #pragma unroll
+        for (int i = 0; i < 16; ++i) first[i] = s0;
+        if (masked) start_masked(s, q_row, key0 + 32 * kb, h, first);  // wave-uniform
+#pragma unroll
         for (int i = 0; i < 16; ++i) {
-          s_acc[i] = s0;
+          s_acc[i] = first[i];
           dp_acc[i] = dp0;
         }
-        if (masked) start_masked(s, q_row, key0 + 32 * kb, h, s_acc);
       };
       auto multiply = [&](auto n) {
         constexpr int last = n + kAhead - 1 < kAll - 1 ? n + kAhead - 1 : kAll - 1;  // newest request
@@ -427,17 +436,19 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load to LDS outlives the workgroup
 
-  if (q_row < T) {
-    bf16_raw* dq_row = dqkv + (int64_t(b) * T + q_row) * tok_stride + int64_t(head) * D;
+  __syncthreads();  // nobody reads the tiles any more
+  using Turn = RowTurn<D, 2>;
+  char* mine = smem + wave * Turn::kBytes;
 #pragma unroll
-    for (int db = 0; db < kDBlocks; ++db)
+  for (int db = 0; db < kDBlocks; ++db)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        u32x2 w = {pack_bf16x2(dq_acc[db][4 * g] * s.scale, dq_acc[db][4 * g + 1] * s.scale),
-                   pack_bf16x2(dq_acc[db][4 * g + 2] * s.scale, dq_acc[db][4 * g + 3] * s.scale)};
-        *reinterpret_cast<u32x2*>(dq_row + db * 32 + 8 * g + 4 * h) = w;
-      }
-  }
+    for (int g = 0; g < 4; ++g) {
+      const u32x2 w = {pack_bf16x2(dq_acc[db][4 * g] * s.scale, dq_acc[db][4 * g + 1] * s.scale),
+                       pack_bf16x2(dq_acc[db][4 * g + 2] * s.scale, dq_acc[db][4 * g + 3] * s.scale)};
+      Turn::put(mine, r, h, db, g, w);
+    }
+  bf16_raw* dq_rows = dqkv + (int64_t(b) * T + q0) * tok_stride + int64_t(head) * D;
+  Turn::store(mine, reinterpret_cast<char*>(dq_rows), tok_stride * 2, T - q0, lane);
 }
 
 }  // namespace

@@ -40,15 +40,15 @@ __device__ __forceinline__ void settle(f32x16 (&acc)[kN]) {
 }
 
 template <int D, bool kDrop, bool kFar>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 64 ? 2 : 1))) void window_dkv_kernel(
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 64 ? (kDrop || kFar ? 2 : 3) : 1))) void window_dkv_kernel(
     const bf16_raw* __restrict__ qkv, const bf16_raw* __restrict__ dout, const float* __restrict__ neg_lse,
     const float* __restrict__ neg_delta, bf16_raw* __restrict__ dqkv, FarSums far, Shape s, DropoutParams drop) {
   constexpr int kKSteps = D / 16;
   constexpr int kDBlocks = D / 32;
   constexpr int kTileBytes = kBN * D * 2;
-  constexpr int kAhead = 6;  // fragments in flight
+  constexpr int kAhead = D == 64 ? 3 : 6;  // fragments in flight
   // [2][Q tile | dO tile], then [2][64 x (-lse / c) | 64 x (-delta)] fp32 row constants
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+  extern __shared__ __attribute__((aligned(256))) char smem[];
   char* row_smem = smem + 4 * kTileBytes;
 
   const int lane = threadIdx.x & 63;
@@ -155,7 +155,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
     asm volatile("" ::"v"(__builtin_bit_cast(u32x4, kf[ks])));
     asm volatile("" ::"v"(__builtin_bit_cast(u32x4, vf[ks])));
   }
-  TileAddr<D> at;
+  TileAddrSmall<D> at;
   at.init(lds_addr(smem), lane);
   unsigned row_at = lds_addr(row_smem) + 16u * (unsigned)h;  // row constants 4 h ..; 8 rows further: + 32 bytes
 
@@ -173,11 +173,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
     constexpr int kChain = subs * kN;
     if constexpr (n < kChain) {
       constexpr int sub = n / kN, m = n % kN;
-      f[n % kAhead] = read16<(m % 2 ? kTileBytes : 0) + sub * 64 * D>(at.row[m / 2]);
+      f[n % kAhead] = read16<(m % 2 ? kTileBytes : 0) + sub * 64 * D>(at.row(m / 2));
     } else if constexpr (n < kChain + subs * kTN) {
       constexpr int sub = (n - kChain) / kTN, m = (n - kChain) % kTN, k = 2 * sub + m / (2 * kDBlocks), db = m / 2 % kDBlocks;
-      tlo[n % kAhead] = read_tr8<(m % 2 ? 0 : kTileBytes) + k * 32 * D>(at.tr[db][0]);
-      thi[n % kAhead] = read_tr8<(m % 2 ? 0 : kTileBytes) + k * 32 * D>(at.tr[db][1]);
+      tlo[n % kAhead] = read_tr8<(m % 2 ? 0 : kTileBytes) + k * 32 * D>(at.tr(db, 0));
+      thi[n % kAhead] = read_tr8<(m % 2 ? 0 : kTileBytes) + k * 32 * D>(at.tr(db, 1));
     }
   };
   // Row constants of a sub-tile: 8 reads, requested ahead like a fragment.
@@ -370,7 +370,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
   for (int j = first_tile; j < end_tile; ++j) {
     const int buf = (j - first_tile) & 1;
     next_tile_ready();
-    if constexpr (kDrop) {
+    if constexpr (kDrop || D == 64) {
       if (j + 1 < end_tile) fetch(j + 1, buf ^ 1);
     } else {
       const bool more = j + 1 < end_tile;
@@ -380,7 +380,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
     }
     const int q0 = j * kBN;
     const int next = buf ? -2 * kTileBytes : 2 * kTileBytes;
-    if constexpr (kDrop) {  // (the pipelined form has no registers left for its masks)
+    // With dropout the pipelined form has no registers left for the masks; with 64 columns three waves on a SIMD, a
+    // sub-tile at a time, beat two that pipeline (8 x 1024, 20 heads, window 256: 48 us against 53).
+    if constexpr (kDrop || D == 64) {
       one(q0);
       at.move(64 * D);
       row_at += 128;
@@ -396,21 +398,23 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
 
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load to LDS outlives the workgroup
   if constexpr (D == 128) settle(dk_acc), settle(dv_acc);
-  if (key < T) {
-    bf16_raw* dk_row = dqkv + (int64_t(b) * T + key) * tok_stride + int64_t(s.H) * D + int64_t(head) * D;
-    bf16_raw* dv_row = dk_row + int64_t(s.H) * D;
+  __syncthreads();  // nobody reads the tiles any more
+  using Turn = RowTurn<D, 2>;
+  char* mine = smem + wave * Turn::kBytes;
+  bf16_raw* dk_rows = dqkv + (int64_t(b) * T + key0) * tok_stride + int64_t(s.H) * D + int64_t(head) * D;
+  auto give = [&](const f32x16 (&acc)[kDBlocks], float factor, bf16_raw* rows) {
 #pragma unroll
     for (int db = 0; db < kDBlocks; ++db)
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        u32x2 wk = {pack_bf16x2(dk_acc[db][4 * g] * s.scale, dk_acc[db][4 * g + 1] * s.scale),
-                    pack_bf16x2(dk_acc[db][4 * g + 2] * s.scale, dk_acc[db][4 * g + 3] * s.scale)};
-        u32x2 wv = {pack_bf16x2(dv_acc[db][4 * g], dv_acc[db][4 * g + 1]),
-                    pack_bf16x2(dv_acc[db][4 * g + 2], dv_acc[db][4 * g + 3])};
-        *reinterpret_cast<u32x2*>(dk_row + db * 32 + 8 * g + 4 * h) = wk;
-        *reinterpret_cast<u32x2*>(dv_row + db * 32 + 8 * g + 4 * h) = wv;
+        const u32x2 w = {pack_bf16x2(acc[db][4 * g] * factor, acc[db][4 * g + 1] * factor),
+                         pack_bf16x2(acc[db][4 * g + 2] * factor, acc[db][4 * g + 3] * factor)};
+        Turn::put(mine, r, h, db, g, w);
       }
-  }
+    Turn::store(mine, reinterpret_cast<char*>(rows), tok_stride * 2, T - key0, lane);
+  };
+  give(dk_acc, s.scale, dk_rows);
+  give(dv_acc, 1.f, dk_rows + int64_t(s.H) * D);
 }
 
 // The far part's chunks: enough workgroups for two per compute unit, at least eight query tiles each (a chunk
