@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import hashlib
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -35,6 +36,9 @@ ARCH = "gfx950"
 # Sources with flags of their own. attention_window*.hip: matrix results in ordinary registers; in accumulator
 # registers every score would be copied across before the vector unit can use it.
 EXTRA_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for name in ("attention_window.hip", "attention_window_dkv.hip")}
+# Sources that read LDS by inline assembly and await the values by count: a register spilled before its value has
+# arrived would be saved too early, so these kernels must not spill at all.
+NO_SPILL = {"attention_window.hip", "attention_window_dkv.hip", "fp8_gemm.hip"}
 ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 
 
@@ -56,6 +60,18 @@ def _hash(paths, flags) -> str:
     return h.hexdigest()
 
 
+def spilling_kernels(remarks: str):
+    """Names of the kernels that use scratch memory, from the compiler's kernel-resource-usage remarks."""
+    name, found = "", []
+    for line in remarks.splitlines():
+        m = re.search(r"remark: .*Function Name: (\S+)", line)
+        name = m.group(1) if m else name
+        m = re.search(r"remark: .*ScratchSize \[bytes/lane\]: (\d+)", line)
+        if m and int(m.group(1)) > 0:
+            found.append(name)
+    return found
+
+
 def _compile(src: Path, cmd_prefix, flags, deps, force, verbose):
     OBJ_DIR.mkdir(parents=True, exist_ok=True)
     rel = src.relative_to(CSRC)
@@ -71,6 +87,9 @@ def _compile(src: Path, cmd_prefix, flags, deps, force, verbose):
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"compilation of {src} failed:\n{proc.stdout}\n{proc.stderr}")
+    if src.name in NO_SPILL and (bad := spilling_kernels(proc.stderr)):
+        obj.unlink()
+        raise RuntimeError(f"{src}: kernels that must not spill registers use scratch memory: {', '.join(bad)}")
     stamp.write_text(digest)
     return obj, True
 
@@ -114,7 +133,8 @@ def build(force: bool = False, verbose: bool = False, sanitize: bool = False) ->
         target.parent.mkdir(parents=True, exist_ok=True)
 
     jobs = int(os.environ.get("MAX_JOBS", "0")) or min(8, os.cpu_count() or 1)
-    tasks = [(s, [hipcc], hip_flags + EXTRA_FLAGS.get(s.name, []), kernel_hdrs) for s in kernel_srcs]
+    own = lambda name: EXTRA_FLAGS.get(name, []) + (["-Rpass-analysis=kernel-resource-usage"] if name in NO_SPILL else [])  # noqa: E731
+    tasks = [(s, [hipcc], hip_flags + own(s.name), kernel_hdrs) for s in kernel_srcs]
     tasks += [(s, [cxx], host_flags, host_hdrs) for s in host_srcs]
     with ThreadPoolExecutor(max_workers=jobs) as pool:
         results = list(pool.map(lambda t: _compile(t[0], t[1], t[2], t[3], force, verbose), tasks))

@@ -123,3 +123,14 @@ def test_refusals_and_plumbing():
     plain, _ = cli.build_model(ap.parse_args(["--model", "llama-tiny"]), "cpu", torch.float32)
     # 12 L d per token and visible key
     assert model_flops_per_token(plain, 128) - model_flops_per_token(model, 128) == 12.0 * 2 * 256 * (128 - 18)
+
+
+def test_build_refuses_spilling_kernels():
+    """The build's check of kernels that must not spill, on the compiler's own wording."""
+    from pytorch_distributed_amd._build import spilling_kernels
+    report = """a.hip:3:1: remark: Function Name: first [-Rpass-analysis=kernel-resource-usage]
+a.hip:3:1: remark:     ScratchSize [bytes/lane]: 0 [-Rpass-analysis=kernel-resource-usage]
+a.hip:9:1: remark: Function Name: second [-Rpass-analysis=kernel-resource-usage]
+a.hip:9:1: remark:     ScratchSize [bytes/lane]: 52 [-Rpass-analysis=kernel-resource-usage]
+"""
+    assert spilling_kernels(report) == ["second"] and spilling_kernels("") == []
