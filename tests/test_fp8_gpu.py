@@ -112,7 +112,8 @@ def test_product(m, n, k, dtype, tiles):
 
 
 @pytest.mark.parametrize("m,n,k", [(8192, 5120, 1280), (8100, 5001, 1300), (16500, 2600, 1400), (2000, 2048, 65536), (2000, 2001, 65536),
-                                   (8192, 1280, 5120), (16384, 1403, 1300), (2000, 1501, 65536)])
+                                   (8192, 1280, 5120), (16384, 1403, 1300), (2000, 1501, 65536),
+                                   (16384, 5120, 100), (16384, 5127, 100)])
 @pytest.mark.parametrize("bias", [None, torch.bfloat16, torch.float32])
 def test_product_of_many_tiles(m, n, k, bias):
     """Sizes at which a workgroup goes through several tiles, and through slices of a long contraction."""
