@@ -670,6 +670,38 @@ struct Fp8Pair {
   at::Tensor q, scale;
 };
 
+// A quantised matrix of `rows` rows of `cols` values by address.
+struct Fp8Buffer {
+  uint8_t *q = nullptr, *scale = nullptr;
+  int64_t rows = 0, cols = 0;
+  bool tiles = false;
+  int64_t ld() const { return round_up(cols, 128); }
+  int64_t ld_scale() const { return round_up((cols + 127) / 128, 4); }
+  int64_t scale_rows() const { return tiles ? (rows + 127) / 128 : rows; }
+  pda::Fp8Operand operand() const { return pda::Fp8Operand{q, scale, ld(), ld_scale(), (int)rows, tiles}; }
+};
+
+// One allocation for what a call needs only until its kernels have run.
+struct Scratch {
+  size_t size = 0;
+  at::Tensor memory;
+  std::vector<std::pair<uint8_t**, size_t>> wanted;
+  void want(uint8_t** p, int64_t bytes) {
+    wanted.emplace_back(p, size);
+    size += (size_t)round_up(bytes, 256);
+  }
+  Fp8Buffer& want(Fp8Buffer& b, int64_t rows, int64_t cols, bool tiles) {
+    b.rows = rows, b.cols = cols, b.tiles = tiles;
+    want(&b.q, rows * b.ld());
+    want(&b.scale, b.scale_rows() * b.ld_scale());
+    return b;
+  }
+  void allocate(const at::TensorOptions& options) {
+    memory = at::empty({(int64_t)size}, options.dtype(at::kByte));
+    for (auto& [p, at] : wanted) *p = memory.data_ptr<uint8_t>() + at;
+  }
+};
+
 // A bf16 / fp32 GPU matrix whose rows are contiguous (any row pitch).
 void check_fp8_source(const at::Tensor& x, const char* name) {
   TORCH_CHECK(x.is_cuda(), "fp8: ", name, " must live on the GPU");
@@ -698,24 +730,12 @@ struct Fp8Quantizer {
 
   // x [R, C] by rows and / or columns, or by tiles (then both layouts share the scales); an output that is not
   // wanted is null. `sums`: fp32 [ceil(R / 128), C] partial column sums (not with tiles).
-  void add(const at::Tensor& x, bool tiles, Fp8Pair* rows, Fp8Pair* cols, at::Tensor* sums) {
-    const int64_t R = x.size(0), C = x.size(1), Rb = (R + 127) / 128, Cb = (C + 127) / 128;
-    const auto q8 = x.options().dtype(at::kFloat8_e4m3fn), u8 = x.options().dtype(at::kByte);
-    if (rows) {
-      rows->q = at::empty({R, Cb * 128}, q8);
-      rows->scale = at::empty({tiles ? Rb : R, round_up(Cb, 4)}, u8);
-    }
-    if (cols) {
-      cols->q = at::empty({C, Rb * 128}, q8);
-      cols->scale = at::empty({tiles ? Cb : C, round_up(Rb, 4)}, u8);
-    }
-    if (sums) *sums = at::empty({Rb, C}, x.options().dtype(at::kFloat));
+  void add(const at::Tensor& x, bool tiles, const Fp8Buffer* rows, const Fp8Buffer* cols, float* sums) {
+    const int64_t R = x.size(0), C = x.size(1);
     if (R == 0 || C == 0) return;  // every output is empty
-    auto bytes = [](const at::Tensor& t) { return reinterpret_cast<uint8_t*>(t.data_ptr()); };
     dtype = dtype_of(x);
-    problems[n++] = {x.data_ptr(), R > 1 ? x.stride(0) : C, (int)R, (int)C, tiles, rows ? bytes(rows->q) : nullptr,
-                     rows ? bytes(rows->scale) : nullptr, cols ? bytes(cols->q) : nullptr,
-                     cols ? bytes(cols->scale) : nullptr, sums ? sums->data_ptr<float>() : nullptr};
+    problems[n++] = {x.data_ptr(), R > 1 ? x.stride(0) : C, (int)R, (int)C, tiles, rows ? rows->q : nullptr,
+                     rows ? rows->scale : nullptr, cols ? cols->q : nullptr, cols ? cols->scale : nullptr, sums};
   }
   void run() {
     if (n == 0) return;
@@ -724,13 +744,25 @@ struct Fp8Quantizer {
   }
 };
 
+// Tensors for a quantised matrix, and where they are.
+Fp8Pair fp8_pair(int64_t rows, int64_t cols, bool tiles, const at::TensorOptions& options, Fp8Buffer* at) {
+  *at = Fp8Buffer{nullptr, nullptr, rows, cols, tiles};
+  Fp8Pair p{at::empty({rows, at->ld()}, options.dtype(at::kFloat8_e4m3fn)), at::empty({at->scale_rows(), at->ld_scale()}, options.dtype(at::kByte))};
+  at->q = reinterpret_cast<uint8_t*>(p.q.data_ptr());
+  at->scale = reinterpret_cast<uint8_t*>(p.scale.data_ptr());
+  return p;
+}
+
 std::vector<at::Tensor> fp8_quantize(const at::Tensor& x, bool want_rows, bool want_cols, bool tiles) {
   check_fp8_source(x, "x");
   TORCH_CHECK(want_rows || want_cols, "fp8_quantize: no output asked for");
   const c10::DeviceGuard guard(x.device());
   Fp8Pair rows, cols;
+  Fp8Buffer r, c;
+  if (want_rows) rows = fp8_pair(x.size(0), x.size(1), tiles, x.options(), &r);
+  if (want_cols) cols = fp8_pair(x.size(1), x.size(0), tiles, x.options(), &c);
   Fp8Quantizer quantizer;
-  quantizer.add(x, tiles, want_rows ? &rows : nullptr, want_cols ? &cols : nullptr, nullptr);
+  quantizer.add(x, tiles, want_rows ? &r : nullptr, want_cols ? &c : nullptr, nullptr);
   quantizer.run();
   std::vector<at::Tensor> out;
   if (want_rows) out.insert(out.end(), {rows.q, rows.scale});
@@ -762,25 +794,21 @@ struct Fp8Products {
   at::TensorOptions partial_options;
 
   // out[M, N] = (out +) bias + x . w^T over K; `out` fresh in `dtype` unless given.
-  at::Tensor add(const Fp8Pair& x, bool x_tiles, const Fp8Pair& w, bool w_tiles, int64_t K, const std::optional<at::Tensor>& bias,
-                 at::ScalarType dtype, const std::optional<at::Tensor>& out, bool accumulate) {
-    const pda::Fp8Operand X = fp8_operand(x.q, x.scale, x_tiles, K, "the left operand");
-    const pda::Fp8Operand W = fp8_operand(w.q, w.scale, w_tiles, K, "the right operand");
-    TORCH_CHECK(x.q.device() == w.q.device(), "fp8_matmul: operands on different devices");
+  at::Tensor add(const pda::Fp8Operand& X, const pda::Fp8Operand& W, int64_t K, const std::optional<at::Tensor>& bias,
+                 const at::TensorOptions& options, const std::optional<at::Tensor>& out, bool accumulate) {
     const int64_t M = X.rows, N = W.rows;
     at::Tensor y;
     if (out.has_value()) {
       y = *out;
-      TORCH_CHECK(y.device() == x.q.device() && y.is_contiguous() && y.numel() == M * N, "fp8_matmul: out must be a contiguous tensor with ",
+      TORCH_CHECK(y.device() == options.device() && y.is_contiguous() && y.numel() == M * N, "fp8_matmul: out must be a contiguous tensor with ",
                   M * N, " elements on the operands' device");
     } else {
       TORCH_CHECK(!accumulate, "fp8_matmul: accumulate needs an out tensor");
-      TORCH_CHECK(dtype == at::kBFloat16 || dtype == at::kFloat, "fp8_matmul: out dtype must be bfloat16 or float32, got ", dtype);
-      y = at::empty({M, N}, x.q.options().dtype(dtype));
+      y = at::empty({M, N}, options);
     }
     const pda::DType out_dtype = dtype_of(y);
     if (bias.has_value())
-      TORCH_CHECK(bias->device() == x.q.device() && bias->is_contiguous() && bias->numel() == N, "fp8_matmul: bias must be a contiguous tensor with ",
+      TORCH_CHECK(bias->device() == options.device() && bias->is_contiguous() && bias->numel() == N, "fp8_matmul: bias must be a contiguous tensor with ",
                   N, " elements on the operands' device");
     const pda::DType bias_dtype = bias.has_value() ? dtype_of(*bias) : pda::kBF16;
     if (M == 0 || N == 0) return y;
@@ -790,7 +818,7 @@ struct Fp8Products {
       return y;
     }
     problems[n++] = {X, W, (int)X.ld, bias.has_value() ? bias->data_ptr() : nullptr, bias_dtype, y.data_ptr(), out_dtype, accumulate, {}, nullptr};
-    partial_options = x.q.options().dtype(at::kFloat);
+    partial_options = options.dtype(at::kFloat);
     return y;
   }
   void run(const pda::Fp8ColumnSums* sums = nullptr) {
@@ -812,8 +840,11 @@ at::Tensor fp8_matmul(const at::Tensor& xq, const at::Tensor& xs, bool x_tiles, 
                       bool w_tiles, int64_t K, const std::optional<at::Tensor>& bias, bool out_f32) {
   TORCH_CHECK(xq.is_cuda(), "fp8_matmul: operands must live on the GPU");
   const c10::DeviceGuard guard(xq.device());
+  const pda::Fp8Operand X = fp8_operand(xq, xs, x_tiles, K, "the left operand");
+  const pda::Fp8Operand W = fp8_operand(wq, ws, w_tiles, K, "the right operand");
+  TORCH_CHECK(xq.device() == wq.device(), "fp8_matmul: operands on different devices");
   Fp8Products products;
-  at::Tensor y = products.add({xq, xs}, x_tiles, {wq, ws}, w_tiles, K, bias, out_f32 ? at::kFloat : at::kBFloat16, std::nullopt, false);
+  at::Tensor y = products.add(X, W, K, bias, xq.options().dtype(out_f32 ? at::kFloat : at::kBFloat16), std::nullopt, false);
   products.run();
   return y;
 }
@@ -828,7 +859,14 @@ std::vector<at::Tensor> fp8_linear_forward(const at::Tensor& x, const at::Tensor
   TORCH_CHECK(x2.scalar_type() == w2.scalar_type() && x2.device() == w2.device() && x2.size(1) == w2.size(1), "fp8_linear: x ",
               x.sizes(), " ", x.scalar_type(), " and weight ", weight.sizes(), " ", weight.scalar_type(), " do not match");
   const c10::DeviceGuard guard(x.device());
-  Fp8Pair xr, xc, wr;
+  const int64_t M = x2.size(0), K = x2.size(1), N = w2.size(0);
+  Fp8Pair kept;
+  Fp8Buffer xr, xc, wr;
+  Scratch scratch;
+  scratch.want(xr, M, K, false);
+  scratch.want(wr, N, K, true);
+  scratch.allocate(x.options());
+  if (keep) kept = fp8_pair(K, M, false, x.options(), &xc);
   Fp8Quantizer quantizer;
   quantizer.add(x2, false, &xr, keep ? &xc : nullptr, nullptr);
   quantizer.add(w2, true, &wr, nullptr, nullptr);
@@ -840,9 +878,9 @@ std::vector<at::Tensor> fp8_linear_forward(const at::Tensor& x, const at::Tensor
   std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
   shape.back() = weight.size(0);
   at::Tensor y = at::empty(shape, x.options());
-  products.add(xr, false, wr, true, x2.size(1), b, x.scalar_type(), y, false);
+  products.add(xr.operand(), wr.operand(), K, b, x.options(), y, false);
   products.run();
-  if (keep) return {y, xc.q, xc.scale};
+  if (keep) return {y, kept.q, kept.scale};
   return {y};
 }
 
@@ -860,31 +898,43 @@ std::vector<at::Tensor> fp8_linear_backward(const at::Tensor& dy, const at::Tens
   TORCH_CHECK(dy.scalar_type() == weight.scalar_type() && dy.device() == weight.device() && w2.size(0) == N,
               "fp8_linear backward: dy ", dy.sizes(), " ", dy.scalar_type(), " and weight ", weight.sizes(), " ", weight.scalar_type(), " do not match");
   const c10::DeviceGuard guard(dy.device());
-  Fp8Pair gr, gc, wc, xc;
-  at::Tensor sums, dx, dw, db, x2;
-  Fp8Quantizer quantizer;
-  if (want_x || want_w || want_b)  // (the bias gradient alone still needs the pass: rows are the cheaper by-product)
-    quantizer.add(g2, false, want_x || !want_w ? &gr : nullptr, want_w ? &gc : nullptr, want_b ? &sums : nullptr);
-  if (want_x) quantizer.add(w2, true, nullptr, &wc, nullptr);
-  if (want_w && x.has_value()) {
+  at::Tensor dx, dw, db, x2;
+  const bool rows = want_x || !want_w;  // (the bias gradient alone still needs the pass: rows are the cheaper by-product)
+  const bool anew = want_w && x.has_value();
+  if (anew) {
     x2 = fp8_source(*x);
     check_fp8_source(x2, "x");
     TORCH_CHECK(x2.size(0) == M && x2.size(1) == K && x2.scalar_type() == dy.scalar_type() && x2.device() == dy.device(),
                 "fp8_linear backward: x ", x->sizes(), " does not match dy ", dy.sizes());
-    quantizer.add(x2, false, nullptr, &xc, nullptr);
   } else if (want_w) {
     TORCH_CHECK(xq.has_value() && xs.has_value(), "fp8_linear backward: the weight gradient needs x");
-    xc = {*xq, *xs};
   }
+  Fp8Buffer gr, gc, wc, xc;
+  uint8_t* sums = nullptr;
+  Scratch scratch;
+  if (rows) scratch.want(gr, M, N, false);
+  if (want_w) scratch.want(gc, N, M, false);
+  if (want_b) scratch.want(&sums, (M + 127) / 128 * N * 4);
+  if (want_x) scratch.want(wc, K, N, true);
+  if (anew) scratch.want(xc, K, M, false);
+  scratch.allocate(dy.options());
+  Fp8Quantizer quantizer;
+  if (want_x || want_w || want_b) quantizer.add(g2, false, rows ? &gr : nullptr, want_w ? &gc : nullptr, (float*)sums);
+  if (want_x) quantizer.add(w2, true, nullptr, &wc, nullptr);
+  if (anew) quantizer.add(x2, false, nullptr, &xc, nullptr);
   quantizer.run();
   Fp8Products products;
   if (want_x) {
-    dx = products.add(gr, false, wc, true, N, std::nullopt, dy.scalar_type(), std::nullopt, false);
+    dx = products.add(gr.operand(), wc.operand(), N, std::nullopt, dy.options(), std::nullopt, false);
     std::vector<int64_t> shape(dy.sizes().begin(), dy.sizes().end());
     shape.back() = K;
     dx = dx.view(shape);
   }
-  if (want_w) dw = products.add(gc, false, xc, false, M, std::nullopt, dy.scalar_type(), w_out, w_accumulate);
+  if (want_w) {
+    const pda::Fp8Operand X = anew ? xc.operand() : fp8_operand(*xq, *xs, false, M, "x");
+    TORCH_CHECK(X.rows == K, "fp8_linear backward: x has ", X.rows, " features, ", K, " expected");
+    dw = products.add(gc.operand(), X, M, std::nullopt, dy.options(), w_out, w_accumulate);
+  }
   pda::Fp8ColumnSums fold{};
   if (want_b) {
     if (b_out.has_value()) {
@@ -895,7 +945,7 @@ std::vector<at::Tensor> fp8_linear_backward(const at::Tensor& dy, const at::Tens
       TORCH_CHECK(!b_accumulate, "fp8_linear backward: accumulating the bias gradient needs its tensor");
       db = at::empty({N}, dy.options());
     }
-    fold = {M > 0 ? sums.data_ptr<float>() : nullptr, (int)((M + 127) / 128), (int)N, db.data_ptr(), dtype_of(db), b_accumulate};
+    fold = {(const float*)sums, (int)((M + 127) / 128), (int)N, db.data_ptr(), dtype_of(db), b_accumulate};
   }
   products.run(want_b && N > 0 ? &fold : nullptr);
   return {dx, dw, db};
