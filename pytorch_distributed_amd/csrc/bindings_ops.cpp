@@ -417,15 +417,16 @@ at::Tensor window_attention_backward(const at::Tensor& qkv, const at::Tensor& ou
               "window attention backward: tensors on different devices");
   const c10::DeviceGuard guard(qkv.device());
   at::Tensor dqkv = at::empty_like(qkv);
-  at::Tensor neg_delta = at::empty_like(neg_lse);
   const size_t bytes = pda::window_attention_backward_workspace_bytes((int)w.B, (int)w.T, (int)w.H, (int)w.D, (int)w.window, (int)w.sinks);
-  at::Tensor workspace;
-  if (bytes) workspace = at::empty({(int64_t)bytes}, qkv.options().dtype(at::kByte));
+  const int64_t delta_bytes = (w.B * w.H * w.T * 4 + 255) / 256 * 256;  // -delta, then the sinks' partial sums
+  at::Tensor scratch = at::empty({delta_bytes + (int64_t)bytes}, qkv.options().dtype(at::kByte));
+  float* neg_delta = reinterpret_cast<float*>(scratch.data_ptr());
+  void* workspace = bytes ? static_cast<char*>(scratch.data_ptr()) + delta_bytes : nullptr;
   pda::window_attention_dq(qkv.data_ptr(), out.data_ptr(), out_rest.data_ptr(), dout.data_ptr(), neg_lse.data_ptr<float>(),
-                           neg_delta.data_ptr<float>(), dqkv.data_ptr(), (int)w.B, (int)w.T, (int)w.H, (int)w.D, (int)w.window,
+                           neg_delta, dqkv.data_ptr(), (int)w.B, (int)w.T, (int)w.H, (int)w.D, (int)w.window,
                            (int)w.sinks, (float)softmax_scale, (float)dropout_p, seed, current_stream());
-  pda::window_attention_dkv(qkv.data_ptr(), dout.data_ptr(), neg_lse.data_ptr<float>(), neg_delta.data_ptr<float>(), dqkv.data_ptr(),
-                            bytes ? workspace.data_ptr() : nullptr, (int)w.B, (int)w.T, (int)w.H, (int)w.D, (int)w.window,
+  pda::window_attention_dkv(qkv.data_ptr(), dout.data_ptr(), neg_lse.data_ptr<float>(), neg_delta, dqkv.data_ptr(),
+                            workspace, (int)w.B, (int)w.T, (int)w.H, (int)w.D, (int)w.window,
                             (int)w.sinks, (float)softmax_scale, (float)dropout_p, seed, current_stream());
   check_launch("window_attention_backward");
   return dqkv;
