@@ -24,8 +24,11 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+import tempfile
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
+
+from ._lds_check import kernels_with_lds_reads, unawaited_reads
 
 PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
@@ -36,9 +39,11 @@ ARCH = "gfx950"
 # Sources with flags of their own. attention_window*.hip: matrix results in ordinary registers; in accumulator
 # registers every score would be copied across before the vector unit can use it.
 EXTRA_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for name in ("attention_window.hip", "attention_window_dkv.hip")}
-# Sources that read LDS by inline assembly and await the values by count: a register spilled before its value has
-# arrived would be saved too early, so these kernels must not spill at all.
+# Sources that read LDS by inline assembly and await the values by count. A register that is copied, spilled or reused
+# before its value has arrived would hold something else, so their assembly is checked (see _lds_check), and of those
+# in NO_SPILL no kernel may spill at all.
 NO_SPILL = {"attention_window.hip", "attention_window_dkv.hip", "fp8_gemm.hip"}
+HAND_READS = NO_SPILL | {"gemm_fused.hip"}
 ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 
 
@@ -61,15 +66,30 @@ def _hash(paths, flags) -> str:
 
 
 def spilling_kernels(remarks: str):
-    """Names of the kernels that use scratch memory, from the compiler's kernel-resource-usage remarks."""
+    """Names of the kernels that use scratch memory or spill vector registers (also into accumulator registers), from
+    the compiler's kernel-resource-usage remarks."""
     name, found = "", []
     for line in remarks.splitlines():
         m = re.search(r"remark: .*Function Name: (\S+)", line)
         name = m.group(1) if m else name
-        m = re.search(r"remark: .*ScratchSize \[bytes/lane\]: (\d+)", line)
-        if m and int(m.group(1)) > 0:
+        m = re.search(r"remark: .*(?:ScratchSize \[bytes/lane\]|VGPRs Spill): (\d+)", line)
+        if m and int(m.group(1)) > 0 and name not in found:
             found.append(name)
     return found
+
+
+def check_hand_reads(source: str, remarks: str, assembly: str) -> None:
+    """Raises if a kernel of ``source`` breaks what its LDS reads by inline assembly rely on, or if the compiler's
+    output does not show the kernels at all. ``remarks``: its kernel-resource-usage remarks (NO_SPILL sources)."""
+    if not kernels_with_lds_reads(assembly):
+        raise RuntimeError(f"{source}: no kernel with LDS reads found in the compiler's assembly; its check would be void")
+    if source in NO_SPILL:
+        if not re.search(r"remark: .*Function Name: ", remarks):
+            raise RuntimeError(f"{source}: no kernel named in the compiler's remarks; their check would be void")
+        if bad := spilling_kernels(remarks):
+            raise RuntimeError(f"{source}: kernels that must not spill registers do: {', '.join(bad)}")
+    if bad := unawaited_reads(assembly):
+        raise RuntimeError(f"{source}: registers touched before the LDS read of them is awaited:\n" + "\n".join(bad))
 
 
 def _compile(src: Path, cmd_prefix, flags, deps, force, verbose):
@@ -81,15 +101,19 @@ def _compile(src: Path, cmd_prefix, flags, deps, force, verbose):
     digest = _hash([src, *deps], [*cmd_prefix, *flags])
     if not force and obj.exists() and stamp.exists() and stamp.read_text() == digest:
         return obj, False
-    cmd = [*cmd_prefix, *flags, "-c", str(src), "-o", str(obj)]
-    if verbose:
-        print("[build]", " ".join(cmd), flush=True)
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        raise RuntimeError(f"compilation of {src} failed:\n{proc.stdout}\n{proc.stderr}")
-    if src.name in NO_SPILL and (bad := spilling_kernels(proc.stderr)):
-        obj.unlink()
-        raise RuntimeError(f"{src}: kernels that must not spill registers use scratch memory: {', '.join(bad)}")
+    hand_reads = src.name in HAND_READS
+    with tempfile.TemporaryDirectory() as temps:  # (the assembler's input, of this very compilation)
+        out = Path(temps) / obj.name if hand_reads else obj
+        cmd = [*cmd_prefix, *flags, *(["--save-temps=obj"] if hand_reads else []), "-c", str(src), "-o", str(out)]
+        if verbose:
+            print("[build]", " ".join(cmd), flush=True)
+        proc = subprocess.run(cmd, capture_output=True, text=True)
+        if proc.returncode != 0:
+            raise RuntimeError(f"compilation of {src} failed:\n{proc.stdout}\n{proc.stderr}")
+        if hand_reads:
+            (listing,) = Path(temps).glob(f"*amdgcn*{ARCH}.s")
+            check_hand_reads(src.name, proc.stderr, listing.read_text())
+            shutil.move(str(out), str(obj))
     stamp.write_text(digest)
     return obj, True
 
@@ -134,7 +158,8 @@ def build(force: bool = False, verbose: bool = False, sanitize: bool = False) ->
 
     jobs = int(os.environ.get("MAX_JOBS", "0")) or min(8, os.cpu_count() or 1)
     own = lambda name: EXTRA_FLAGS.get(name, []) + (["-Rpass-analysis=kernel-resource-usage"] if name in NO_SPILL else [])  # noqa: E731
-    tasks = [(s, [hipcc], hip_flags + own(s.name), kernel_hdrs) for s in kernel_srcs]
+    check = PKG_DIR / "_lds_check.py"
+    tasks = [(s, [hipcc], hip_flags + own(s.name), kernel_hdrs + ([check] if s.name in HAND_READS else [])) for s in kernel_srcs]
     tasks += [(s, [cxx], host_flags, host_hdrs) for s in host_srcs]
     with ThreadPoolExecutor(max_workers=jobs) as pool:
         results = list(pool.map(lambda t: _compile(t[0], t[1], t[2], t[3], force, verbose), tasks))
