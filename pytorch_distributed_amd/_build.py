@@ -43,7 +43,7 @@ EXTRA_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for name in ("attent
 # before its value has arrived would hold something else, so their assembly is checked (see _lds_check), and of those
 # in NO_SPILL no kernel may spill at all.
 NO_SPILL = {"attention_window.hip", "attention_window_dkv.hip", "fp8_gemm.hip"}
-HAND_READS = NO_SPILL | {"gemm_fused.hip"}
+HAND_READS = NO_SPILL | {"gemm_fused.hip", "gemm_wgrad.hip"}
 ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
 
 

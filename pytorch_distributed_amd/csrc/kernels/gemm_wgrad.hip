@@ -136,7 +136,6 @@ __device__ __forceinline__ void stage_half(const bf16_raw* src, char* tile, int 
   __builtin_amdgcn_global_load_lds((gptr_t*)src, (lptr_t*)dst, 16, 0, 0);
 }
 
-template <int kMode>
 __global__ __launch_bounds__(kThreads) void wgrad_kernel(const bf16_raw* __restrict__ A, int64_t lda,
                                                          const bf16_raw* __restrict__ B, int64_t ldb,
                                                          float* __restrict__ c_partial,
@@ -247,14 +246,12 @@ __global__ __launch_bounds__(kThreads) void wgrad_kernel(const bf16_raw* __restr
       // those rows has landed AND every wave is done reading stage t-1, whose slot the next
       // issue overwrites.
       const int younger = n_steps - 1 - t;
-      if (kMode == 1) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      else if (younger >= 2) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+      if (younger >= 2) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
       else if (younger == 1) asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
       else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       __builtin_amdgcn_sched_barrier(0);
-      if (kMode != 1 && t + kStages - 1 < n_steps) issue(t + kStages - 1, (u + kStages - 1) % kStages);
-      if (kMode == 2) continue;
+      if (t + kStages - 1 < n_steps) issue(t + kStages - 1, (u + kStages - 1) % kStages);
 
       const unsigned a_tile = smem_base + u * kStageBytes;
       const unsigned b_tile = a_tile + kTileBytes;
@@ -269,13 +266,11 @@ __global__ __launch_bounds__(kThreads) void wgrad_kernel(const bf16_raw* __restr
         fl[b] = tr_read<8192>(b_tile + b_base[b]);
         fh[b] = tr_read<12288>(b_tile + b_base[b]);
       }
+      asm volatile("s_waitcnt lgkmcnt(12)" ::: "memory");  // k-step 0 fragments (read a stage ago)
       u32x4 bias_rows[2];
       if (do_bias) {  // column sums of the A tile: thread owns chunk (tid & 31) of rows (tid >> 5) + 16 i
         bias_rows[0] = b128_read<0>(a_tile + bias_off);
         bias_rows[1] = b128_read<8192>(a_tile + bias_off);
-        asm volatile("s_waitcnt lgkmcnt(14)" ::: "memory");  // k-step 0 fragments (read a stage ago)
-      } else {
-        asm volatile("s_waitcnt lgkmcnt(12)" ::: "memory");
       }
       __builtin_amdgcn_sched_barrier(0);
       bf16x8 af[4], bfr[2];
@@ -288,12 +283,9 @@ __global__ __launch_bounds__(kThreads) void wgrad_kernel(const bf16_raw* __restr
 #pragma unroll
         for (int b = 0; b < 2; ++b) acc[a][b] = mfma32(af[a], bfr[b], acc[a][b]);
       __builtin_amdgcn_sched_barrier(0);
-      if (younger >= 1) {  // k-step 0 of stage t+1 (landed before this stage's barrier)
-        read_k0((u + 1) % kStages);
-        asm volatile("s_waitcnt lgkmcnt(12)" ::: "memory");
-      } else {
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // k-step 1 fragments and the bias rows
+      __builtin_amdgcn_sched_barrier(0);
+      if (younger >= 1) read_k0((u + 1) % kStages);  // k-step 0 of stage t+1 (landed before this stage's barrier)
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int a = 0; a < 4; ++a)
@@ -311,6 +303,7 @@ __global__ __launch_bounds__(kThreads) void wgrad_kernel(const bf16_raw* __restr
     }
   }
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
   __syncthreads();  // the ring is reused below
 
   // ---- epilogue: fp32 partial tile ------------------------------------------------------
@@ -530,6 +523,10 @@ __global__ __launch_bounds__(kThreads4) void wgrad_kernel4(const bf16_raw* __res
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < 16; ++i) frag_read(0, 0, 0, i);
+    // Awaited here: the compiler copies these registers on its way into the loops, and their wait is inside.
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int x = 0; x < 4; ++x) asm volatile("" : "+v"(al[0][x]), "+v"(ah[0][x]), "+v"(bl[0][x]), "+v"(bh[0][x]));
   }
 
 #ifdef PDA_WGRAD_STAMPS
@@ -624,11 +621,10 @@ __global__ __launch_bounds__(kThreads4) void wgrad_kernel4(const bf16_raw* __res
         }
       }
     }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // the tail's dummy loads and reads
   };
   if (do_bias) main_loop(std::true_type{});
   else main_loop(std::false_type{});
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the tail's dummy loads
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   __syncthreads();  // the ring is reused below
 #ifdef PDA_WGRAD_STAMPS
   const unsigned long long t_loop_end = __builtin_amdgcn_s_memtime();
@@ -850,9 +846,14 @@ __global__ __launch_bounds__(kThreads4) void wgrad_kernel16(const bf16_raw* __re
       read_a(0, 0, x, 0);
       read_a(0, 0, x, 1);
     }
+    // Awaited here: the compiler copies these registers on its way into the loops, and their wait is inside.
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
     if (do_bias) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) bias_read(0, j);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 
@@ -898,10 +899,10 @@ __global__ __launch_bounds__(kThreads4) void wgrad_kernel16(const bf16_raw* __re
         });
       });
     }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // the tail's dummy loads and reads
   };
   if (do_bias) main_loop(std::true_type{});
   else main_loop(std::false_type{});
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // the tail's dummy loads and reads
   __syncthreads();  // the ring is reused below
 
   // acc[a][b] register e of lane (g, c): row i = 16*(8*wi + a) + c, column j = 16*(8*wj + b) + 4*g + e.
@@ -1005,28 +1006,26 @@ bool wgrad_supported(int M, int I, int J) {
 void wgrad_gemm(const void* A, int64_t lda, const void* B, int64_t ldb, float* c_partial,
                 float* bias_partial, int M, int I, int J, int S, hipStream_t stream) {
   const int n_tasks = ((I + kTile - 1) / kTile) * ((J + kTile - 1) / kTile) * S;
-  static int mode = -1, waves = 4, mfma = 32, order = -1;
-  if (mode < 0) {
+  static bool configured = false;
+  static int waves = 4, mfma = 32, order = -1;
+  if (!configured) {
     (void)hipFuncSetAttribute((const void*)wgrad_kernel4<0>, hipFuncAttributeMaxDynamicSharedMemorySize, kStages * kStageBytes);
     (void)hipFuncSetAttribute((const void*)wgrad_kernel16<0>, hipFuncAttributeMaxDynamicSharedMemorySize, kStages * kStageBytes);
     const char* mf = getenv("PDA_WGRAD_MFMA");  // 16 selects the 16 x 16 x 32 four-wave kernel (A/B measurements)
     mfma = mf ? atoi(mf) : 32;
     const char* w = getenv("PDA_WGRAD_WAVES");  // 8 selects the eight-wave kernel (A/B measurements)
     waves = w ? atoi(w) : 4;
-    (void)hipFuncSetAttribute((const void*)wgrad_kernel<0>, hipFuncAttributeMaxDynamicSharedMemorySize, kStages * kStageBytes);
-    (void)hipFuncSetAttribute((const void*)wgrad_kernel<1>, hipFuncAttributeMaxDynamicSharedMemorySize, kStages * kStageBytes);
-    (void)hipFuncSetAttribute((const void*)wgrad_kernel<2>, hipFuncAttributeMaxDynamicSharedMemorySize, kStages * kStageBytes);
+    (void)hipFuncSetAttribute((const void*)wgrad_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kStages * kStageBytes);
     const char* o = getenv("PDA_WGRAD_ORDER");  // 0 / 1 force the j-fastest / i-fastest tile order (A/B measurements)
     order = o ? atoi(o) : -1;
-    const char* e = getenv("PDA_WGRAD_MODE");
-    mode = e ? atoi(e) : 0;
+    configured = true;
   }
-  if (waves == 4 && mode == 0 && mfma == 16) {
+  if (waves == 4 && mfma == 16) {
     hipLaunchKernelGGL(wgrad_kernel16<0>, dim3((unsigned)n_tasks), dim3(kThreads4), kStages * kStageBytes, stream,
                        (const bf16_raw*)A, lda, (const bf16_raw*)B, ldb, c_partial, bias_partial, M, I, J, S);
     return;
   }
-  if (waves == 4 && mode == 0) {
+  if (waves == 4) {
     const int tiles_i = (I + kTile - 1) / kTile, tiles_j = (J + kTile - 1) / kTile;
     const int i_fast = order < 0 ? (tiles_j > tiles_i) : order;
     hipLaunchKernelGGL(wgrad_kernel4<0>, dim3((unsigned)n_tasks), dim3(kThreads4), kStages * kStageBytes, stream,
@@ -1034,8 +1033,7 @@ void wgrad_gemm(const void* A, int64_t lda, const void* B, int64_t ldb, float* c
                        WgradSegments{});
     return;
   }
-  auto kern = mode == 1 ? wgrad_kernel<1> : mode == 2 ? wgrad_kernel<2> : wgrad_kernel<0>;
-  hipLaunchKernelGGL(kern, dim3((unsigned)n_tasks), dim3(kThreads), kStages * kStageBytes, stream,
+  hipLaunchKernelGGL(wgrad_kernel, dim3((unsigned)n_tasks), dim3(kThreads), kStages * kStageBytes, stream,
                      (const bf16_raw*)A, lda, (const bf16_raw*)B, ldb, c_partial, bias_partial, M, I, J, S);
 }
 

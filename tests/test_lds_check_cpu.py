@@ -1,4 +1,6 @@
 """The build's check of kernels that read LDS by inline assembly: on written-out assembly, right and wrong."""
+import re
+
 import pytest
 
 from pytorch_distributed_amd import _build
@@ -68,3 +70,13 @@ def test_the_build_refuses():
         _build.check_hand_reads("gemm_fused.hip", "", "")
     with pytest.raises(RuntimeError, match="before the LDS read of them is awaited"):
         _build.check_hand_reads("gemm_fused.hip", "", kernel(READ, USE, "s_endpgm"))
+
+
+def test_every_source_with_such_reads_is_checked():
+    read = re.compile(r'asm volatile\("[^"]*ds_(read|load|bpermute)')
+    kernels = _build.CSRC / "kernels"
+    headers = [h.name for h in kernels.glob("*.h") if read.search(h.read_text())]
+    for src in sorted(kernels.glob("*.hip")):
+        text = src.read_text()
+        if read.search(text) or any(f'#include "{h}"' in text for h in headers):
+            assert src.name in _build.HAND_READS, src.name
