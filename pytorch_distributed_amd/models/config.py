@@ -81,16 +81,20 @@ class LlamaConfig:
         return self
 
 
-def check_block_options(config) -> None:
-    """Refuses values of ``linear_precision`` / ``sliding_window`` / ``attention_sinks`` that mean nothing."""
-    if config.linear_precision not in ("bf16", "fp8"):
-        raise ValueError(f"linear_precision must be 'bf16' or 'fp8', got {config.linear_precision!r}")
-    if config.sliding_window is not None and int(config.sliding_window) < 1:
-        raise ValueError(f"sliding_window must be at least 1 (or None), got {config.sliding_window}")
-    if int(config.attention_sinks) < 0:
-        raise ValueError(f"attention_sinks must not be negative, got {config.attention_sinks}")
-    if config.attention_sinks and config.sliding_window is None:
+def block_options(config):
+    """``(linear_precision, sliding_window, attention_sinks)`` of a model's blocks; a configuration without these
+    fields has their defaults. Refuses values that mean nothing."""
+    precision = getattr(config, "linear_precision", "bf16")
+    window, sinks = getattr(config, "sliding_window", None), getattr(config, "attention_sinks", 0)
+    if precision not in ("bf16", "fp8"):
+        raise ValueError(f"linear_precision must be 'bf16' or 'fp8', got {precision!r}")
+    if window is not None and int(window) < 1:
+        raise ValueError(f"sliding_window must be at least 1 (or None), got {window}")
+    if int(sinks) < 0:
+        raise ValueError(f"attention_sinks must not be negative, got {sinks}")
+    if sinks and window is None:
         raise ValueError("attention_sinks needs a sliding_window (without one every earlier key is visible)")
+    return precision, window, sinks
 
 
 _GPT2 = {

@@ -42,7 +42,7 @@ from torch import nn
 from .. import ops
 from ..ops.regen import GeluRegen, NormRegen
 from ..utils.recompute import recompute
-from .config import check_block_options, GPT2Config, get_config, normalize_gpt2_config
+from .config import GPT2Config, block_options, get_config, normalize_gpt2_config
 
 
 class MyGPT2Attention(nn.Module):
@@ -57,9 +57,8 @@ class MyGPT2Attention(nn.Module):
         self.c_attn = nn.Linear(self.embed_dim, 3 * self.embed_dim, bias=True)
         self.c_proj = nn.Linear(self.embed_dim, self.embed_dim, bias=True)
         self.attn_pdrop = float(config.attn_pdrop)
-        check_block_options(config)
-        self.linear = ops.fp8_linear if config.linear_precision == "fp8" else ops.linear
-        self.sliding_window, self.attention_sinks = config.sliding_window, config.attention_sinks
+        precision, self.sliding_window, self.attention_sinks = block_options(config)
+        self.linear = ops.fp8_linear if precision == "fp8" else ops.linear
         self.resid_dropout = nn.Dropout(p=config.resid_pdrop)
 
     def forward(self, hidden_states: torch.Tensor, apply_dropout: bool = True, input_regen=None) -> torch.Tensor:
@@ -89,8 +88,7 @@ class MyGPT2MLP(nn.Module):
         self.c_fc = nn.Linear(self.embed_dim, 4 * self.embed_dim, bias=True)
         self.c_proj = nn.Linear(4 * self.embed_dim, self.embed_dim, bias=True)
         self.dropout = nn.Dropout(p=config.resid_pdrop)
-        check_block_options(config)
-        self.linear_precision = config.linear_precision
+        self.linear_precision, _, _ = block_options(config)
 
     def forward(self, hidden_states: torch.Tensor, apply_dropout: bool = True, input_regen=None,
                 regen_activation: bool = False) -> torch.Tensor:

@@ -20,7 +20,7 @@ from torch import nn
 from .. import _ext, ops
 from ..ops.regen import NormRegen, SwigluRegen
 from ..utils.recompute import recompute
-from .config import LlamaConfig, check_block_options, get_config
+from .config import LlamaConfig, block_options, get_config
 
 
 class RMSNorm(nn.Module):
@@ -96,9 +96,8 @@ class LlamaAttention(nn.Module):
         super().__init__()
         self.num_heads = config.n_head
         self.head_dim = config.head_dim
-        check_block_options(config)
-        self.linear = ops.fp8_linear if config.linear_precision == "fp8" else ops.linear
-        self.sliding_window, self.attention_sinks = config.sliding_window, config.attention_sinks
+        precision, self.sliding_window, self.attention_sinks = block_options(config)
+        self.linear = ops.fp8_linear if precision == "fp8" else ops.linear
         self.wqkv = nn.Linear(config.n_embd, 3 * config.n_embd, bias=False)
         self.c_proj = nn.Linear(config.n_embd, config.n_embd, bias=False)
 
@@ -114,8 +113,7 @@ class LlamaAttention(nn.Module):
 class LlamaMLP(nn.Module):
     def __init__(self, config: LlamaConfig):
         super().__init__()
-        check_block_options(config)
-        self.linear = ops.fp8_linear if config.linear_precision == "fp8" else ops.linear
+        self.linear = ops.fp8_linear if block_options(config)[0] == "fp8" else ops.linear
         self.gate_up = nn.Linear(config.n_embd, 2 * config.intermediate_size, bias=False)
         self.down = nn.Linear(config.intermediate_size, config.n_embd, bias=False)
 

@@ -24,7 +24,7 @@ def model_flops_per_token(model, seq_len: int) -> float:
     if cfg is None:
         return 0.0
     if getattr(cfg, "sliding_window", None) is not None:
-        seq_len = min(seq_len, cfg.sliding_window + cfg.attention_sinks)
+        seq_len = min(seq_len, cfg.sliding_window + getattr(cfg, "attention_sinks", 0))
     if hasattr(cfg, "intermediate_size"):  # Llama-style: 4 d^2 + 3 d f per layer, untied head
         n_mm = cfg.n_layer * (4 * cfg.n_embd ** 2 + 3 * cfg.n_embd * cfg.intermediate_size) \
             + cfg.n_embd * cfg.vocab_size

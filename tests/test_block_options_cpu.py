@@ -1,6 +1,7 @@
 """8-bit linear layers and sliding-window attention inside the models, on the CPU reference paths."""
 import copy
 import dataclasses
+import types
 
 import pytest
 import torch
@@ -134,3 +135,17 @@ a.hip:9:1: remark: Function Name: second [-Rpass-analysis=kernel-resource-usage]
 a.hip:9:1: remark:     ScratchSize [bytes/lane]: 52 [-Rpass-analysis=kernel-resource-usage]
 """
     assert spilling_kernels(report) == ["second"] and spilling_kernels("") == []
+
+
+def test_a_configuration_without_the_options_has_their_defaults():
+    """Any object with the fields that the models read is a configuration; the options are optional."""
+    fields = {k: v for k, v in dataclasses.asdict(get_config("llama-tiny")).items()
+              if k not in ("linear_precision", "sliding_window", "attention_sinks")}
+    cfg = types.SimpleNamespace(**fields, head_dim=get_config("llama-tiny").head_dim)
+    torch.manual_seed(0)
+    model = LlamaForCausalLM(cfg, activation_checkpoint="none")
+    x, y = batch()
+    assert torch.equal(model(x, y), build("llama-tiny")(x, y))
+    assert model_flops_per_token(model, 64) == model_flops_per_token(build("llama-tiny"), 64)
+    cfg.sliding_window = 16
+    assert model_flops_per_token(model, 64) == model_flops_per_token(build("llama-tiny", sliding_window=16), 64)
