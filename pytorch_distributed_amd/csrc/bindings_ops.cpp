@@ -850,6 +850,26 @@ at::Tensor fp8_matmul(const at::Tensor& xq, const at::Tensor& xs, bool x_tiles, 
   return y;
 }
 
+// What the products of one call (at most two) are planned as: {tile, slices} each, for {M, N, K, fp32 result, accumulate}.
+std::vector<std::vector<int64_t>> fp8_plan(const std::vector<std::vector<int64_t>>& products) {
+  TORCH_CHECK(products.size() <= 2, "fp8_plan: at most two products share a call, got ", products.size());
+  pda::Fp8GemmProblem problems[2] = {};
+  for (size_t i = 0; i < products.size(); ++i) {
+    const auto& p = products[i];
+    TORCH_CHECK(p.size() == 5 && p[0] >= 1 && p[1] >= 1 && p[2] >= 1 && p[0] <= (1 << 22) && p[1] <= (1 << 22) && p[2] <= (1 << 22),
+                "fp8_plan: a product is {M, N, K, fp32, accumulate} with sizes between 1 and 2^22");
+    problems[i].x.rows = (int)p[0];
+    problems[i].w.rows = (int)p[1];
+    problems[i].K = (int)round_up(p[2], 128);
+    problems[i].out_dtype = p[3] ? pda::kF32 : pda::kBF16;
+    problems[i].accumulate = p[4] != 0;
+  }
+  pda::fp8_gemm_plan(problems, (int)products.size());
+  std::vector<std::vector<int64_t>> plans;
+  for (size_t i = 0; i < products.size(); ++i) plans.push_back({problems[i].plan.tile, problems[i].plan.slices});
+  return plans;
+}
+
 // y = x . w^T + bias with x [..., K] quantised by rows and w [N, K] by tiles. `keep`: also x quantised by
 // columns (from the same read of x), which is all that the weight gradient needs of it.
 std::vector<at::Tensor> fp8_linear_forward(const at::Tensor& x, const at::Tensor& weight, const std::optional<at::Tensor>& bias,
@@ -1152,6 +1172,7 @@ void bind_ops(py::module_& m) {
   m.def("fp8_quantize", &fp8_quantize, py::arg("x"), py::arg("rows"), py::arg("columns"), py::arg("tiles"));
   m.def("fp8_matmul", &fp8_matmul, py::arg("xq"), py::arg("xs"), py::arg("x_tiles"), py::arg("wq"), py::arg("ws"),
         py::arg("w_tiles"), py::arg("K"), py::arg("bias"), py::arg("out_f32"));
+  m.def("fp8_plan", &fp8_plan, py::arg("products"));
   m.def("fp8_linear", &fp8_linear, py::arg("x"), py::arg("weight"), py::arg("bias"));
   m.def("fp8_linear_forward", &fp8_linear_forward, py::arg("x"), py::arg("weight"), py::arg("bias"), py::arg("keep"));
   m.def("fp8_linear_backward", &fp8_linear_backward, py::arg("dy"), py::arg("weight"), py::arg("x"), py::arg("xq"), py::arg("xs"),

@@ -757,9 +757,12 @@ static Work work_of(const Fp8GemmPlan& plan, const Fp8GemmProblem& p) {
   return Work{tiles_of(plan.tile, p.x.rows, p.w.rows) * plan.slices, std::min(plan.steps_per_slice, p.K / kStageK)};
 }
 static float fold_time(const Fp8GemmPlan& plan, const Fp8GemmProblem& p) {
-  return plan.slices == 1 ? 0.f : 3.f + float(p.x.rows) * p.w.rows * (8.f * plan.slices + 2.f) / 4.5e6f;
+  if (plan.slices == 1 && !p.accumulate) return 0.f;
+  const float out = (p.out_dtype == kF32 ? 4.f : 2.f) * (p.accumulate ? 2.f : 1.f);
+  return 3.f + float(p.x.rows) * p.w.rows * (8.f * plan.slices + out) / 4.5e6f;
 }
 
+// (of one launch: the problems are widened both or neither)
 static float time_of(const Fp8GemmPlan* plans, const Fp8GemmProblem* problems, int n) {
   Work work[2] = {};
   float t = 0.f;
@@ -795,14 +798,25 @@ static Choice choose(int tile, const Fp8GemmProblem* problems, int n) {
   return best;
 }
 
+// No large tile: widened products, or what its epilogue's 32-bit offsets and bias loads do not reach.
+static bool small_only(const Fp8GemmProblem& p) {
+  return p.out_dtype == kF32 || p.w.rows > (1 << 20) || reinterpret_cast<uintptr_t>(p.bias) % 4 != 0;
+}
+
+// Two products share a launch, and so a tile, if they take the same kernel. Where they do not (a weight gradient into
+// an fp32 buffer, which is widened and tied to the small tile, beside a bf16 input gradient), each is planned by itself.
 void fp8_gemm_plan(Fp8GemmProblem* problems, int n) {
-  bool small = false;  // no large tile: widened products, or what its epilogue's 32-bit offsets and bias loads do not reach
-  for (int i = 0; i < n; ++i) {
-    const Fp8GemmProblem& p = problems[i];
-    small |= p.out_dtype == kF32 || p.w.rows > (1 << 20) || reinterpret_cast<uintptr_t>(p.bias) % 4 != 0;
+  auto alike = [&]() {
+    return (problems[0].out_dtype == kF32) == (problems[1].out_dtype == kF32) && small_only(problems[0]) == small_only(problems[1]);
+  };
+  if (n == 2 && !alike()) {
+    fp8_gemm_plan(problems, 1);
+    fp8_gemm_plan(problems + 1, 1);
+    return;
   }
+  if (n == 0) return;
   Choice best = choose(128, problems, n);
-  if (!small) {
+  if (!small_only(problems[0])) {
     for (int tile : {192, 256}) {
       const Choice big = choose(tile, problems, n);
       if (big.time < best.time) best = big;
