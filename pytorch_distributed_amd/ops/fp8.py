@@ -42,6 +42,12 @@ BLOCK = 128
 _DTYPES = (torch.bfloat16, torch.float32)
 
 
+def _exp2(e: torch.Tensor) -> torch.Tensor:
+    """2^e in fp32 for whole numbers from -127 to 127, exact on every device (``torch.ldexp`` and ``exp2`` are off by
+    the last bit at some exponents on the GPU): the number's own bits."""
+    return torch.where(e >= -126, (e + 127) << 23, 1 << 22).to(torch.int32).view(torch.float32)
+
+
 class Fp8Matrix:
     """A quantised matrix of ``rows`` x ``cols`` values.
 
@@ -75,7 +81,7 @@ class Fp8Matrix:
         if self.tiles:
             e = e.repeat_interleave(BLOCK, 0)[: self.rows]
         v = self.q.to(torch.float32).view(self.rows, blocks, BLOCK)
-        return torch.ldexp(v, e.unsqueeze(2)).view(self.rows, blocks * BLOCK)[:, : self.cols]
+        return (v * _exp2(e).unsqueeze(2)).view(self.rows, blocks * BLOCK)[:, : self.cols]
 
 
 # --------------------------------------------------------------------------- references
@@ -92,7 +98,7 @@ def _quantize_reference(v: torch.Tensor, rows_per_block: int) -> Tuple[torch.Ten
     a = v.abs()
     a = torch.where(torch.isfinite(a), a, torch.zeros_like(a))
     e = _exponent_reference(a.amax((1, 3)) if v.numel() else a.new_zeros(v.shape[0], blocks))
-    q = torch.ldexp(v, -e[:, None, :, None])
+    q = v * _exp2(-e)[:, None, :, None]
     q = torch.where(torch.isfinite(v), q, torch.full_like(q, float("nan"))).to(torch.float8_e4m3fn)
     scale = F.pad((e + 127).to(torch.uint8), (0, -blocks % 4))
     return q.view(q.shape[0] * rows_per_block, blocks * BLOCK)[:rows], scale
