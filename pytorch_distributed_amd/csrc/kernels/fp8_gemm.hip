@@ -30,7 +30,7 @@
 // fp32 results. The 8-bit matrix instructions align the 64 products of a call to the largest of them and drop
 // bits: measured (random e4m3 operands) up to 1.3e-4 of sum |x w|, 5e-5 in norm, whatever the contraction's
 // length. Next to a bf16 result's rounding (1.7e-3) that is nothing; an fp32 result is computed with kWide
-// instead: fragments widened to bf16 on the way to v_mfma_f32_32x32x16_bf16, scale included (exact), whose
+// instead: fragments widened to bf16 on the way to v_mfma_f32_32x32x16_bf16, scale included (exact: see widen2), whose
 // sums are good to 6e-8, at half the matrix rate (1003 x 1601 x 777: 12.1 us).
 //
 // Few output tiles (weight gradients, few tokens): the contraction is cut into slices of whole 512-value
@@ -88,8 +88,10 @@ __device__ __forceinline__ f32x16 mfma_scaled(i32x8 a, i32x8 b, f32x16 c, uint32
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, 0, 0, 0, (int)sa, 0, (int)sb);
 }
 
-// Two of the e4m3 values of `v` (its lower or upper half) times 2^(byte - 127) as bf16: exact, e4m3 has 4
-// significant bits and bf16 its scale's range.
+// Two of the e4m3 values of `v` (its lower or upper half) times 2^(byte - 127) as bf16: exact for bytes of 3 and more
+// (e4m3 has 4 significant bits and its smallest number is 2^-9; bf16's is 2^-133, and the matrix instruction takes
+// subnormal operands). At bytes 0 to 2, blocks whose largest magnitude is at most 448 * 2^-125, it rounds to multiples of
+// 2^-133.
 template <bool kHigh>
 __device__ __forceinline__ uint32_t widen2(uint32_t v, uint32_t byte) {
   const bf16x2 p = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v, __uint_as_float(byte << 23), kHigh);

@@ -42,7 +42,7 @@ __device__ __forceinline__ uint32_t scale_byte(float amax) {
   return uint32_t(max(e, 0));
 }
 
-// 2^-(byte - 127). Bytes run from 0 to 248 (max float: 2^127 * 2 / 448), so the result is a normal float.
+// 2^-(byte - 127). Bytes run from 0 to 247 (the largest float, just below 2^128, takes 2^120), so the result is a normal float.
 __device__ __forceinline__ float inverse_scale(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
 
 __device__ __forceinline__ uint32_t pack_fp8x4(float a, float b, float c, float d) {

@@ -19,7 +19,7 @@ The pieces are public: ``quantize_fp8`` (layouts in its docstring) and ``fp8_mat
 quantises a weight once and multiplies by it many times.
 
 Numbers: an element is off by at most half a step of e4m3, 2^-4 of its own size as long as it is within
-2^-14 of its block's largest, so a product of random operands is off by some 4 % of its own size. Values
+2^-13 of its block's largest, so a product of random operands is off by some 4 % of its own size. Values
 far below their block's largest become subnormal or zero. An infinity or NaN of the input is a NaN of the
 quantised matrix in its place alone and takes no part in the scale: it shows up in the products that read
 it. Gradients are those of the product of the quantised operands with respect to these operands (the
@@ -52,8 +52,8 @@ class Fp8Matrix:
     """A quantised matrix of ``rows`` x ``cols`` values.
 
     ``q``: float8_e4m3fn ``[rows, ceil(cols / 128) * 128]``, zeros behind column ``cols``. ``scale``:
-    uint8 ``[rows, S]`` — or ``[ceil(rows / 128), S]`` with ``tiles`` — the byte ``b`` of a block standing for
-    ``2^(b - 127)``; S is the number of blocks in a row rounded up to 4 (the padding is not read)."""
+    uint8 ``[rows, S]`` — or ``[ceil(rows / 128), S]`` with ``tiles`` — the byte ``b`` of a block, at most 254,
+    standing for ``2^(b - 127)``; S is the number of blocks in a row rounded up to 4 (the padding is not read)."""
 
     __slots__ = ("q", "scale", "cols", "tiles")
 
@@ -156,7 +156,8 @@ def quantize_fp8(x: torch.Tensor, blocks: str = "rows") -> Union[Fp8Matrix, Tupl
 def fp8_matmul(a: Fp8Matrix, b: Fp8Matrix, bias: Optional[torch.Tensor] = None,
                out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``a @ b.T + bias`` for ``a [M, K]`` and ``b [N, K]``, accumulated in fp32, as bf16 or fp32 ``[M, N]``.
-    ``bias``: bf16 or fp32 ``[N]``. Not differentiable (``fp8_linear`` is)."""
+    An fp32 result takes what its operands hold in blocks of scale bytes 0 to 2 (magnitudes below 2^-116) to multiples
+    of 2^-133 first. ``bias``: bf16 or fp32 ``[N]``. Not differentiable (``fp8_linear`` is)."""
     if a.cols != b.cols:
         raise ValueError(f"fp8_matmul: contraction lengths differ, {a.cols} and {b.cols}")
     if out_dtype not in _DTYPES:

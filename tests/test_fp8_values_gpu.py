@@ -40,3 +40,28 @@ def test_reference_on_the_gpu_agrees_with_the_kernel_at_ties(blocks, monkeypatch
     for a, b in zip(kernel, ops.quantize_fp8(x, blocks)):
         blocks_in_row = -(-a.cols // 128)
         assert torch.equal(a.q.view(torch.uint8), b.q.view(torch.uint8)) and torch.equal(a.scale[:, :blocks_in_row], b.scale[:, :blocks_in_row])
+
+
+@pytest.mark.parametrize("byte", [0, 1, 2, 3, 9, 60])
+@pytest.mark.parametrize("left", [True, False])
+def test_products_at_the_smallest_scales(byte, left):
+    """One operand at the smallest scales, the other so large that the product is an ordinary number. To bf16 the scale
+    is applied inside the instruction; to fp32 the operand is widened to bf16 first, whose smallest number is 2^-133:
+    exact from byte 3 on, below that each element is off by half of it at the most."""
+    g = torch.Generator(device=DEV).manual_seed(byte)
+    m, n, k = 70, 100, 300
+    small = torch.randint(-60, 61, (m, k), generator=g, device=DEV).float() * 2.0 ** -9  # subnormal and small e4m3 numbers
+    q = torch.zeros(m, 384, device=DEV)
+    q[:, :k] = small
+    a = ops.Fp8Matrix(q.to(torch.float8_e4m3fn), torch.full((m, 4), byte, dtype=torch.uint8, device=DEV), k)
+    b = ops.quantize_fp8(torch.randn(n, k, generator=g, device=DEV) * 2.0 ** 112)
+    x, w = a.q.double()[:, :k] * 2.0 ** (byte - 127), b.dequantize().double()
+    want, size = x @ w.t().contiguous(), x.abs() @ w.abs().t().contiguous()
+    if not left:
+        a, b, want, size = b, a, want.t(), size.t()
+    y = ops.fp8_matmul(a, b, None, torch.bfloat16).double()
+    assert ((y - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -12 * size).all()
+    y = ops.fp8_matmul(a, b, None, torch.float32).double()
+    rounded = 2.0 ** -134 * w.abs().sum(1) if byte < 3 else torch.zeros(n, dtype=torch.float64, device=DEV)
+    rounded = rounded[None, :] if left else rounded[:, None]
+    assert ((y - want).abs() <= 2.0 ** -24 * want.abs() + (k / 16 + 16) * 2.0 ** -23 * size + rounded * 1.01).all()
