@@ -257,7 +257,8 @@ def fp8_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     if bias is not None and (bias.dtype != x.dtype or bias.device != x.device or tuple(bias.shape) != (weight.shape[0],)):
         raise ValueError(f"fp8_linear: bias must be {x.dtype} [{weight.shape[0]}] on {x.device}, "
                          f"got {bias.dtype} {tuple(bias.shape)} on {bias.device}")
-    if (regen is None and _ext.use_hip(x) and getattr(weight, "_pda_grad_sink", None) is None
-            and getattr(bias, "_pda_grad_sink", None) is None):
+    # (without grad mode nobody asks for gradients, whoever owns them, and nothing is kept of x)
+    if _ext.use_hip(x) and (not torch.is_grad_enabled() or (regen is None and getattr(weight, "_pda_grad_sink", None) is None
+                                                            and getattr(bias, "_pda_grad_sink", None) is None)):
         return _ext.require().fp8_linear(x, weight, bias)
     return _Fp8LinearFn.apply(x, weight, bias, regen)

@@ -63,3 +63,24 @@ def test_buffers_repeat_bit_for_bit(dtype):
         assert all(torch.equal(a, c) for a, c in zip(got, want))
         assert all(torch.equal(a, c) for a, c in zip(want, twice()))
         torch.cuda.synchronize()
+
+
+def test_evaluation_keeps_nothing():
+    """Without grad mode a layer whose gradients have an owner makes no copy of its input, in values or in memory."""
+    m, n, k = 4096, 256, 2048
+    x, w, b, _ = fp8.layer_case(m, n, k, torch.bfloat16)
+    x = x.detach()
+
+    def peak():
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        with torch.no_grad():
+            y = ops.fp8_linear(x, w, b)
+        return y, torch.cuda.max_memory_allocated() - before
+
+    want, plain = peak()
+    w._pda_grad_sink = b._pda_grad_sink = lambda: None
+    got, owned = peak()
+    assert torch.equal(got, want) and not got.requires_grad
+    assert owned <= plain  # (the copy alone is m * k bytes, 8 MiB)
