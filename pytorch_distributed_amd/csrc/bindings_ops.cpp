@@ -369,10 +369,13 @@ WindowShape check_window(const at::Tensor& qkv, int64_t num_heads, int64_t windo
   WindowShape w{qkv.size(0), qkv.size(1), num_heads, qkv.size(2) / (3 * num_heads), window, sinks};
   TORCH_CHECK(w.D == 64 || w.D == 128, "window attention: head_dim must be 64 or 128, got ", w.D);
   TORCH_CHECK(w.B >= 1 && w.T >= 1, "window attention: empty input");
-  TORCH_CHECK(w.T <= (1 << 30) && (w.T / 128 + 1) * w.B * w.H < (int64_t(1) << 31) && 64 * qkv.size(2) * 2 < (int64_t(1) << 31),
-              "window attention: sizes exceed the kernels' 32-bit indices");
   w.window = std::min(window, w.T);
   w.sinks = std::min(sinks, w.T);
+  // (a launch takes less than 2^32 threads: workgroups of 256, one for 128 rows of a head, in the backward one for 32 sinks)
+  const int64_t most = std::max((w.T + 127) / 128, w.window < w.T ? (w.sinks + 31) / 32 : 0);
+  TORCH_CHECK(w.T <= (1 << 30) && w.B < (1 << 30) && w.H < (1 << 30) && w.B * w.H < (int64_t(1) << 24) &&
+                  most * w.B * w.H < (int64_t(1) << 24) && 64 * qkv.size(2) * 2 < (int64_t(1) << 31),
+              "window attention: sizes exceed the kernels' 32-bit indices");
   return w;
 }
 

@@ -68,3 +68,14 @@ def test_dropout_over_many_tiles(B, T, H, D, window, sinks):
     win.check(g, wg, tg)
     again, g2 = win.run(qkv, dout, H, window, sinks, dropout_p=p, training=True, seed=seed)
     assert torch.equal(out, again) and torch.equal(g, g2)
+
+
+def test_most_heads_of_one_launch():
+    """As many single-token sequences as one launch has workgroups for, where the result is V itself; one more is refused."""
+    n = 2 ** 24
+    qkv = torch.empty(n, 1, 192, device=DEV, dtype=torch.bfloat16)
+    qkv.view(-1, 2 ** 20, 192).copy_(win.inputs(1, 2 ** 20, 1, 64)[0])
+    with pytest.raises(RuntimeError, match="32-bit indices"):
+        ops.window_attention(qkv, 1, 1)
+    out = ops.window_attention(qkv[1:], 1, 1)
+    assert torch.equal(out, qkv[1:, :, 128:])
