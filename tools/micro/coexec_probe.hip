@@ -1,7 +1,7 @@
 // Can the matrix pipe and the vector ALU of one SIMD work for two different waves at once? One
 // workgroup of 8 waves per CU (2 per SIMD): waves 0-3 issue independent v_mfma_f32_32x32x16_bf16
 // back to back, waves 4-7 run the element-wise part of an attention-backward tile (32 v_exp_f32,
-// 16 v_pk_mul_f32, 16 v_cvt_pk_bf16_f32 per trip). Each kind is timed alone and together.
+// 32 v_mul_f32, 16 v_cvt_pk_bf16_f32 per trip). Each kind is timed alone and together.
 // Build: hipcc --offload-arch=gfx950 -O3 -o tools/micro/bin/coexec_probe tools/micro/coexec_probe.hip
 #include <hip/hip_runtime.h>
 #include <stdint.h>

@@ -22,7 +22,7 @@ typedef __attribute__((ext_vector_type(4))) float f32x4;
   } while (0)
 
 // kExtra: what is issued between two MFMAs: 0 nothing, 1 two ds_read_b64 (consumed a loop trip later), 2 two v_add_u32,
-// 3 four s_add_u32, 4 one ds_read_b64, 5 four ds_read_b64, 6 four v_exp_f32, 7 two v_pk_mul_f32 + two v_cvt_pk_bf16_f32,
+// 3 four s_add_u32, 4 one ds_read_b64, 5 four ds_read_b64, 6 four v_exp_f32, 7 four v_mul_f32 + two v_cvt_pk_bf16_f32,
 // 8 all eight of 6 and 7
 template <int kShape, int kExtra>  // 32: 32x32x16, 16: 16x16x32
 __global__ __launch_bounds__(512) void probe(float* out, unsigned long long* cycles, int iters) {
@@ -45,8 +45,7 @@ __global__ __launch_bounds__(512) void probe(float* out, unsigned long long* cyc
   uint64_t rd[4] = {0, 0, 0, 0};
   unsigned va = threadIdx.x, vb = 1, sa = iters, sb = 3;
   float fx[8] = {0, 0, 0, 0, 0, 0, 0, 0}, fy[4] = {-0.5f, -1.5f, -2.5f, -0.25f * threadIdx.x};
-  typedef __attribute__((ext_vector_type(2))) float f32x2;
-  f32x2 px[4] = {{0, 0}, {0, 0}, {0, 0}, {0, 0}}, py[2] = {{1.5f, 2.5f}, {0.5f, 0.25f}};
+  float px[8] = {0, 0, 0, 0, 0, 0, 0, 0}, py[4] = {1.5f, 2.5f, 0.5f, 0.25f};
   unsigned cv[4] = {0, 0, 0, 0};
   __syncthreads();
   const unsigned long long t0 = __builtin_amdgcn_s_memtime();
@@ -59,7 +58,7 @@ __global__ __launch_bounds__(512) void probe(float* out, unsigned long long* cyc
       if constexpr (kExtra == 1 || kExtra == 4 || kExtra == 5) {
         constexpr int n = kExtra == 1 ? 2 : kExtra == 4 ? 1 : 4;
 #pragma unroll
-        for (int q = 0; q < n; ++q) asm volatile("ds_read_b64 %0, %1 offset:%2" : "=v"(rd[q]) : "v"(lds_at), "n"(512 * 0) : "memory");
+        for (int q = 0; q < n; ++q) asm volatile("ds_read_b64 %0, %1 offset:%2" : "+v"(rd[q]) : "v"(lds_at), "n"(512 * 0) : "memory");  // (in / out: the register stays the read's)
       }
       if constexpr (kExtra == 2) {
         asm volatile("v_add_u32 %0, %0, %1" : "+v"(va) : "v"(vb));
@@ -69,17 +68,17 @@ __global__ __launch_bounds__(512) void probe(float* out, unsigned long long* cyc
 #pragma unroll
         for (int q = 0; q < 4; ++q) asm volatile("v_exp_f32 %0, %1" : "=v"(fx[4 * (k & 1) + q]) : "v"(fy[q]));
       }
-      if constexpr (kExtra == 7) {  // two v_pk_mul_f32 and two v_cvt_pk_bf16_f32, all to different registers
-        asm volatile("v_pk_mul_f32 %0, %1, %2" : "=v"(px[2 * (k & 1)]) : "v"(py[0]), "v"(py[1]));
-        asm volatile("v_pk_mul_f32 %0, %1, %2" : "=v"(px[2 * (k & 1) + 1]) : "v"(py[1]), "v"(py[0]));
+      if constexpr (kExtra == 7) {  // four v_mul_f32 and two v_cvt_pk_bf16_f32, all to different registers
+#pragma unroll
+        for (int q = 0; q < 4; ++q) asm volatile("v_mul_f32 %0, %1, %2" : "=v"(px[4 * (k & 1) + q]) : "v"(py[q]), "v"(py[q ^ 1]));
         asm volatile("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(cv[2 * (k & 1)]) : "v"(fy[0]), "v"(fy[1]));
         asm volatile("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(cv[2 * (k & 1) + 1]) : "v"(fy[2]), "v"(fy[3]));
       }
-      if constexpr (kExtra == 8) {  // eight: 4 v_exp_f32, 2 v_pk_mul_f32, 2 v_cvt_pk_bf16_f32
+      if constexpr (kExtra == 8) {  // ten: 4 v_exp_f32, 4 v_mul_f32, 2 v_cvt_pk_bf16_f32
 #pragma unroll
         for (int q = 0; q < 4; ++q) asm volatile("v_exp_f32 %0, %1" : "=v"(fx[4 * (k & 1) + q]) : "v"(fy[q]));
-        asm volatile("v_pk_mul_f32 %0, %1, %2" : "=v"(px[2 * (k & 1)]) : "v"(py[0]), "v"(py[1]));
-        asm volatile("v_pk_mul_f32 %0, %1, %2" : "=v"(px[2 * (k & 1) + 1]) : "v"(py[1]), "v"(py[0]));
+#pragma unroll
+        for (int q = 0; q < 4; ++q) asm volatile("v_mul_f32 %0, %1, %2" : "=v"(px[4 * (k & 1) + q]) : "v"(py[q]), "v"(py[q ^ 1]));
         asm volatile("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(cv[2 * (k & 1)]) : "v"(fy[0]), "v"(fy[1]));
         asm volatile("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(cv[2 * (k & 1) + 1]) : "v"(fy[2]), "v"(fy[3]));
       }
@@ -97,9 +96,9 @@ __global__ __launch_bounds__(512) void probe(float* out, unsigned long long* cyc
   const unsigned long long t1 = __builtin_amdgcn_s_memtime();
   float s = float(rd[0] + rd[1] + rd[2] + rd[3]) + float(va + vb + sa + sb);
 #pragma unroll
-  for (int q = 0; q < 8; ++q) s += fx[q];
+  for (int q = 0; q < 8; ++q) s += fx[q] + px[q];
 #pragma unroll
-  for (int q = 0; q < 4; ++q) s += px[q][0] + px[q][1] + float(cv[q]);
+  for (int q = 0; q < 4; ++q) s += float(cv[q]);
 #pragma unroll
   for (int k = 0; k < 8; ++k) s += acc[k][0] + acc[k][kElems - 1];
   out[blockIdx.x * blockDim.x + threadIdx.x] = s;
@@ -142,13 +141,13 @@ int main() {
   run<32, 2>("2 v_add_u32,", out, cyc);
   run<32, 3>("4 s_add_u32,", out, cyc);
   run<32, 6>("4 v_exp_f32,", out, cyc);
-  run<32, 7>("2 pk_mul + 2 cvt_pk,", out, cyc);
-  run<32, 8>("4 exp+2 pk_mul+2 cvt,", out, cyc);
+  run<32, 7>("4 mul + 2 cvt_pk,", out, cyc);
+  run<32, 8>("4 exp+4 mul+2 cvt,", out, cyc);
   run<32, 9>("8 v_fma_f32,", out, cyc);
   run<33, 0>("nothing,", out, cyc);
   run<33, 2>("2 v_add_u32,", out, cyc);
   run<33, 9>("8 v_fma_f32,", out, cyc);
-  run<33, 8>("4 exp+2 pk_mul+2 cvt,", out, cyc);
+  run<33, 8>("4 exp+4 mul+2 cvt,", out, cyc);
   run<33, 1>("2 ds_read_b64,", out, cyc);
   run<16, 0>("nothing,", out, cyc);
   run<16, 4>("1 ds_read_b64,", out, cyc);

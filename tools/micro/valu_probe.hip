@@ -1,5 +1,5 @@
 // Vector-instruction cost probe for gfx950: cycles (s_memtime) per iteration of the element-wise
-// part of an attention-backward tile — 32 v_exp_f32, 16 packed (or 32 scalar) multiplies, 16
+// part of an attention-backward tile — 32 v_exp_f32, 32 multiplies (of pairs, or one by one), 16
 // v_cvt_pk_bf16_f32 — run from registers by 1, 2 or 3 waves per SIMD, one workgroup per CU.
 // Build: hipcc --offload-arch=gfx950 -O3 -o tools/micro/bin/valu_probe tools/micro/valu_probe.hip
 #include <hip/hip_runtime.h>
@@ -19,8 +19,8 @@ typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
     }                                                                           \
   } while (0)
 
-// kMode: 0 = 32 exp; 1 = 32 exp + 16 pk_mul; 2 = 32 exp + 32 scalar mul; 3 = mode 1 + 16 cvt_pk; 4 = 32 fma only;
-// 5 = 16 pk_mul only; 6 = 16 cvt only
+// kMode: 0 = 32 exp; 1 = 32 exp + 16 multiplies of pairs; 2 = 32 exp + 32 single multiplies; 3 = mode 1 + 16 cvt_pk; 4 = 32 fma only;
+// 5 = 16 multiplies of pairs only; 6 = 16 cvt only
 template <int kMode>
 __global__ void probe(float* out, unsigned long long* cycles, int iters) {
   float s[32], d[32];
@@ -90,11 +90,11 @@ int main() {
   CHECK(hipMalloc(&out, 256 * 1024 * sizeof(float)));
   CHECK(hipMalloc(&cyc, 16 * sizeof(unsigned long long)));
   run<0>("32 v_exp_f32", out, cyc);
-  run<1>("32 v_exp_f32 + 16 v_pk_mul_f32", out, cyc);
+  run<1>("32 v_exp_f32 + 16 x 2 multiplies", out, cyc);
   run<2>("32 v_exp_f32 + 32 v_mul_f32", out, cyc);
-  run<3>("32 v_exp_f32 + 16 v_pk_mul_f32 + 16 v_cvt_pk", out, cyc);
+  run<3>("32 v_exp_f32 + 16 x 2 multiplies + 16 v_cvt_pk", out, cyc);
   run<4>("32 v_fma_f32", out, cyc);
-  run<5>("16 v_pk_mul_f32", out, cyc);
+  run<5>("16 x 2 multiplies", out, cyc);
   run<6>("16 v_cvt_pk_bf16_f32", out, cyc);
   return 0;
 }
