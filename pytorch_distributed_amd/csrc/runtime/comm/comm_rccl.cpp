@@ -172,19 +172,8 @@ class RcclCommunicator final : public Communicator {
     // The streams are created BEFORE the library initialises, at normal priority. Measured on this
     // stack (ROCm 7.0 runtime, RCCL 2.26): the first high-priority stream created after
     // ncclCommInitRank stops draining as soon as it exchanges more than a couple of event fences with
-    // the default stream (tools/micro/comm_chain.py reproduces it; streams created before the
-    // initialisation, or at normal priority, do not show it). PDA_COMM_STREAM_PRIORITY=high opts into
-    // high-priority streams (still created first).
-    {
-      const char* pr = std::getenv("PDA_COMM_STREAM_PRIORITY");
-      const bool high = pr != nullptr && pr[0] == 'h';
-      int least = 0, greatest = 0;
-      PDA_HIP(hipDeviceGetStreamPriorityRange(&least, &greatest));
-      for (int q = 0; q < 2; ++q) {
-        if (high) PDA_HIP(hipStreamCreateWithPriority(&streams_[q], hipStreamNonBlocking, greatest));
-        else PDA_HIP(hipStreamCreateWithFlags(&streams_[q], hipStreamNonBlocking));
-      }
-    }
+    // the default stream; streams created before the initialisation, or at normal priority, do not.
+    for (int q = 0; q < 2; ++q) PDA_HIP(hipStreamCreateWithFlags(&streams_[q], hipStreamNonBlocking));
     comms_[0].store(init_library_communicator());
     if (dual) {
       comms_[1].store(init_library_communicator());
