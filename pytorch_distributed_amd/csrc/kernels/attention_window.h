@@ -23,10 +23,6 @@ __device__ __forceinline__ void static_for(F&& f) {
   }
 }
 
-__device__ __forceinline__ unsigned lds_addr(const char* p) {
-  return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
-}
-
 // ---- LDS reads in flight. An asm output counts as written at once, so nothing may touch it before wait_for
 // (which ties the registers to the wait): a kernel that uses these must not spill, its register budget is chosen so. kYounger: reads requested after the one awaited.
 template <int kOff>

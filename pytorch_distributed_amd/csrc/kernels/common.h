@@ -166,6 +166,11 @@ __device__ __forceinline__ float block_max(float v, float* scratch) {
   return r;
 }
 
+// A shared-memory pointer as the LDS byte address that inline assembly takes.
+__device__ __forceinline__ unsigned lds_addr(const char* p) {
+  return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
+}
+
 __host__ __device__ __forceinline__ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 }  // namespace pda

@@ -54,10 +54,6 @@ constexpr int kGroupStages = 8;             // stages whose scales are fetched t
 constexpr int kSlots = 256;                 // workgroups of the 256 tile at once: one per compute unit
 constexpr int kGroupM = 4;                  // token tiles walked together by consecutive tasks
 
-__device__ __forceinline__ unsigned lds_addr(const char* p) {
-  return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
-}
-
 // LDS reads through inline assembly: the compiler would wait for all global_load_lds in flight before an
 // ordinary LDS read. Completion is awaited by the stage body before the values are used.
 template <int kOff>

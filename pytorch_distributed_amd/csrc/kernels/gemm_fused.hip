@@ -63,10 +63,6 @@ constexpr int kStageBytes = 2 * kTileBytes;        // X slab | W slab
 constexpr int kLoadsPerStage = 4;                  // global_load_lds per wave and stage (2 X + 2 W)
 constexpr int kGroupM = 4;                         // token tiles walked together by consecutive tasks
 
-__device__ __forceinline__ unsigned lds_addr(const char* p) {
-  return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
-}
-
 // LDS reads go through inline asm: with global_load_lds in flight the compiler cannot prove an
 // ordinary LDS read does not alias their destination and would drain the whole queue in front of
 // it. Completion is awaited explicitly (counted lgkmcnt + a scheduling fence) before the MFMAs.

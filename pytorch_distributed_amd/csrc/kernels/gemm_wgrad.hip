@@ -62,10 +62,6 @@ __device__ __forceinline__ int wg_tile_off(int row, int chunk) {
 // destination and drains the whole queue (s_waitcnt vmcnt(0)) in front of it, which would
 // serialise the ring. The asm reads are invisible to that bookkeeping; their completion is
 // awaited explicitly (counted s_waitcnt lgkmcnt + a scheduling fence) before the MFMAs.
-__device__ __forceinline__ unsigned lds_addr(const char* p) {
-  return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)p;
-}
-
 template <int kOff>
 __device__ __forceinline__ s16x4 tr_read(unsigned addr) {
   s16x4 v;
