@@ -41,7 +41,7 @@
 // the kernel below in its straightforward form; its interleaved form did not survive the compiler's register
 // allocation (16-register accumulator tuples stay live whole, 28 spills). Not shipped; the analysis stands.
 // The kernels keep the vector part small: both row constants ride in the accumulators' initial values and the
-// softmax scale is folded into an operand once per kernel, so a probability costs one v_exp_f32, half a packed
+// softmax scale is folded into an operand once per kernel, so a probability costs one v_exp_f32, a
 // multiply and one or two halves of a v_cvt_pk_bf16_f32.
 #include "attention_common.h"
 #include "pda_kernels.h"
@@ -135,7 +135,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
   // The softmax works in exp2 units: P = exp2(c S - LSE log2 e), c = scale * log2 e. Both constants are
   // moved out of the tile loop: this lane's Q fragments are multiplied by c once (rounded to bf16 like
   // Q itself) and -LSE log2 e is the initial value of the S accumulator, so the MFMA chain ends as the
-  // exponent and a probability costs one v_exp_f32 (a packed multiply-add per pair less per tile).
+  // exponent and a probability costs one v_exp_f32 (a multiply-add less).
   const float c = scale * kLog2e;
 #pragma unroll
   for (int ks = 0; ks < kKSteps; ++ks)
@@ -215,8 +215,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
 #endif
       const int key0 = j * kBN;
       const bool diag = key0 + kBN - 1 > q0;  // wave-uniform
-      // dS^T = P^T (dP^T - delta), without the softmax scale. Two elements per packed fp32
-      // instruction; the causal mask is only evaluated on tiles that straddle the diagonal.
+      // dS^T = P^T (dP^T - delta), without the softmax scale; the causal mask is only evaluated on tiles that straddle the diagonal.
       auto softmax_grad = [&](auto masked) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
@@ -445,7 +444,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
         }
         const bool diag = qs < key0 + 31;          // wave-uniform: some (q, key) pairs are masked
         const bool tail = qs + 31 >= T;            // wave-uniform: padding queries in this sub-tile
-        // P and dS = P (dP - delta), two elements per packed fp32 instruction. Only tiles on the
+        // P and dS = P (dP - delta). Only tiles on the
         // diagonal or past the end of the sequence evaluate the mask (separate code paths:
         // folded into one, the per-element compares ran on every tile).
         // Dropout: the forward multiplied V by keep * P / (1 - p). dV takes that dropped P; dS is

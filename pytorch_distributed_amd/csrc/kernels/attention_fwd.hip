@@ -130,8 +130,8 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
       // ---- causal mask (only on tiles that straddle the diagonal), row maximum, exponentials ------
       // The softmax works in exp2 units: p = exp2(c * s - m) with c = scale * log2(e) and m the
       // running maximum of c * s. The maximum is taken over the RAW scores (c > 0) and the scale is
-      // folded into one packed fused multiply-add per pair in front of the exponential, so a score
-      // costs max3 (1/2), fma (1/2), exp2 (1), sum (1/2), convert (1/2) instructions.
+      // folded into the fused multiply-add in front of the exponential, so a score
+      // costs max3 (1/2), fma (1), exp2 (1), sum (1), convert (1/2) instructions.
       // max3() is inline assembly and the compiler inserts no MFMA -> VALU wait states for inline
       // assembly, so the wait is explicit: 24 idle cycles cover the 8-pass MFMA that wrote last
       // (the fence also ties the accumulators to this point of the instruction stream).

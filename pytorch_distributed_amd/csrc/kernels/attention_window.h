@@ -23,8 +23,9 @@ __device__ __forceinline__ void static_for(F&& f) {
   }
 }
 
-// ---- LDS reads in flight. An asm output counts as written at once, so nothing may touch it before wait_for
-// (which ties the registers to the wait): a kernel that uses these must not spill, its register budget is chosen so. kYounger: reads requested after the one awaited.
+// ---- LDS reads in flight. An asm output counts as written at once, so nothing may touch it before wait_for (which
+// ties the registers to the wait). A kernel that uses these must not spill, its register budget is chosen so, and the
+// build checks the compiler's output for both. kYounger: reads requested after the one awaited.
 template <int kOff>
 __device__ __forceinline__ u32x4 read16(unsigned addr) {
   u32x4 v;

@@ -28,7 +28,7 @@
 // as the products. Results leave through LDS in whole rows (dK / dV 48 -> 43 there).
 //
 // Every sum has one owner and a fixed order: results repeat bit for bit. Probabilities and their gradients
-// are rounded to bf16 as operands of the second products (relative 2^-9 each, averaged by the sums); scores,
+// are rounded to bf16 as operands of the second products (by at most 2^-8 of each, averaged by the sums); scores,
 // softmax statistics and accumulators are fp32, and unlike the causal backward no operand is pre-scaled.
 // Dropout draws the causal kernels' mask (a function of seed, head, query and key).
 #include "attention_window.h"
