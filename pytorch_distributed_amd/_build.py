@@ -28,7 +28,7 @@ import tempfile
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
-from ._lds_check import kernels_with_lds_reads, unawaited_reads
+from ._asm_check import early_products, kernels_with_lds_reads, unawaited_reads
 
 PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
@@ -40,8 +40,8 @@ ARCH = "gfx950"
 # registers every score would be copied across before the vector unit can use it.
 EXTRA_FLAGS = {name: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for name in ("attention_window.hip", "attention_window_dkv.hip")}
 # Sources that read LDS by inline assembly and await the values by count. A register that is copied, spilled or reused
-# before its value has arrived would hold something else, so their assembly is checked (see _lds_check), and of those
-# in NO_SPILL no kernel may spill at all.
+# before its value has arrived would hold something else, so their assembly is checked (see _asm_check, also for
+# matrix products written as inline assembly), and of those in NO_SPILL no kernel may spill at all.
 NO_SPILL = {"attention_window.hip", "attention_window_dkv.hip", "fp8_gemm.hip"}
 HAND_READS = NO_SPILL | {"gemm_fused.hip", "gemm_wgrad.hip"}
 ROCM = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
@@ -90,6 +90,8 @@ def check_hand_reads(source: str, remarks: str, assembly: str) -> None:
             raise RuntimeError(f"{source}: kernels that must not spill registers do: {', '.join(bad)}")
     if bad := unawaited_reads(assembly):
         raise RuntimeError(f"{source}: registers touched before the LDS read of them is awaited:\n" + "\n".join(bad))
+    if bad := early_products(assembly):
+        raise RuntimeError(f"{source}: registers touched before the matrix product into them is done:\n" + "\n".join(bad))
 
 
 def _compile(src: Path, cmd_prefix, flags, deps, force, verbose):
@@ -158,7 +160,7 @@ def build(force: bool = False, verbose: bool = False, sanitize: bool = False) ->
 
     jobs = int(os.environ.get("MAX_JOBS", "0")) or min(8, os.cpu_count() or 1)
     own = lambda name: EXTRA_FLAGS.get(name, []) + (["-Rpass-analysis=kernel-resource-usage"] if name in NO_SPILL else [])  # noqa: E731
-    check = PKG_DIR / "_lds_check.py"
+    check = PKG_DIR / "_asm_check.py"
     tasks = [(s, [hipcc], hip_flags + own(s.name), kernel_hdrs + ([check] if s.name in HAND_READS else [])) for s in kernel_srcs]
     tasks += [(s, [cxx], host_flags, host_hdrs) for s in host_srcs]
     with ThreadPoolExecutor(max_workers=jobs) as pool:

@@ -28,15 +28,14 @@ struct FarSums {
 };
 
 // acc += a b with acc in accumulator registers. The compiler does not know that this is a matrix instruction: the
-// nop covers operands that vector instructions have just written, settle() whatever reads acc after the last one;
-// products of one acc are at least four apart, and nothing else touches it in between.
+// nop covers operands that vector instructions have just written, settle() whatever reads acc after the last one, the
+// compiler's own copies included (so a loop that they may leave or enter settles in every trip; the build checks what
+// the compiler made of it); products of one acc are at least four apart, and nothing else touches it in between.
 __device__ __forceinline__ void mfma32_acc(bf16x8 a, bf16x8 b, f32x16& acc) {
   asm volatile("s_nop 1\n\tv_mfma_f32_32x32x16_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
 }
-template <int kN>
-__device__ __forceinline__ void settle(f32x16 (&acc)[kN]) {
-#pragma unroll
-  for (int i = 0; i < kN; ++i) asm volatile("s_nop 15\n\ts_nop 15" : "+a"(acc[i]));
+__device__ __forceinline__ void settle(f32x16 (&a)[4], f32x16 (&b)[4]) {
+  asm volatile("s_nop 15\n\ts_nop 3" : "+a"(a[0]), "+a"(a[1]), "+a"(a[2]), "+a"(a[3]), "+a"(b[0]), "+a"(b[1]), "+a"(b[2]), "+a"(b[3]));
 }
 
 template <int D, bool kDrop, bool kFar>
@@ -323,9 +322,9 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
       fetch(min(j + 1, end_tile - 1), 1);
       next_tile_ready();
       one((j + (wave >> 1)) * kBN + 32 * (wave & 1));
+      if constexpr (D == 128) settle(dk_acc, dv_acc);
       __syncthreads();  // everyone has read the two tiles
     }
-    if constexpr (D == 128) settle(dk_acc), settle(dv_acc);
     // sum over the waves: 2, 3 -> 0, 1, then 1 -> 0 (each through its own place in LDS: 64 lanes x 16 floats a block)
     float* red = reinterpret_cast<float*>(smem);
     auto give = [&](int slot) {
@@ -397,7 +396,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(D == 6
   }
 
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no load to LDS outlives the workgroup
-  if constexpr (D == 128) settle(dk_acc), settle(dv_acc);
+  if constexpr (D == 128) settle(dk_acc, dv_acc);
   __syncthreads();  // nobody reads the tiles any more
   using Turn = RowTurn<D, 2>;
   char* mine = smem + wave * Turn::kBytes;

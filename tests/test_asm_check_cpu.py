@@ -1,10 +1,11 @@
-"""The build's check of kernels that read LDS by inline assembly: on written-out assembly, right and wrong."""
+"""The build's check of kernels with LDS reads and matrix products by inline assembly: on written-out assembly, right
+and wrong."""
 import re
 
 import pytest
 
 from pytorch_distributed_amd import _build
-from pytorch_distributed_amd._lds_check import kernels_with_lds_reads, unawaited_reads
+from pytorch_distributed_amd._asm_check import WAIT_STATES, early_products, kernels_with_lds_reads, unawaited_reads
 
 
 def kernel(*lines, name="_Zkernel"):
@@ -70,10 +71,33 @@ def test_the_build_refuses():
         _build.check_hand_reads("gemm_fused.hip", "", "")
     with pytest.raises(RuntimeError, match="before the LDS read of them is awaited"):
         _build.check_hand_reads("gemm_fused.hip", "", kernel(READ, USE, "s_endpgm"))
+    with pytest.raises(RuntimeError, match="before the matrix product into them is done"):
+        _build.check_hand_reads("gemm_fused.hip", "", kernel(READ, "s_waitcnt lgkmcnt(0)", *INLINE, "v_accvgpr_read_b32 v2, a15", "s_endpgm"))
 
 
-def test_every_source_with_such_reads_is_checked():
-    read = re.compile(r'asm volatile\("[^"]*ds_(read|load|bpermute)')
+INLINE = [";;#ASMSTART", "v_mfma_f32_32x32x16_bf16 a[0:15], v[4:7], v[8:11], a[0:15]", ";;#ASMEND"]
+
+
+@pytest.mark.parametrize("touch", ["v_accvgpr_read_b32 v2, a15", "v_accvgpr_mov_b32 a40, a3", "v_accvgpr_write_b32 a0, 0", "buffer_store_dwordx4 a[12:15], v0, s[0:3], 0 offen",
+                                   "v_mfma_f32_32x32x16_bf16 a[16:31], a[0:3], v[8:11], a[16:31]"])
+def test_a_product_touched_too_early_is_found(touch):
+    fill = ["v_add_u32_e32 v40, v41, v42"] * (WAIT_STATES - 17)
+    assert len(early_products(kernel(*INLINE, "s_nop 15", *fill[:-1], touch, "s_endpgm"))) == 1
+    assert early_products(kernel(*INLINE, "s_nop 15", *fill, "s_nop 0", touch, "s_endpgm")) == []
+    # on one path
+    assert len(early_products(kernel(*INLINE, "s_cbranch_scc1 .L1", "s_nop 15", "s_nop 15", ".L1:", touch, "s_endpgm"))) == 1
+    # around a loop
+    assert len(early_products(kernel(".L1:", touch, *INLINE, "s_cbranch_scc1 .L1", "s_endpgm"))) == 1
+
+
+def test_products_into_one_accumulator_follow_each_other():
+    assert early_products(kernel(*INLINE, *INLINE, "s_nop 15", "s_nop 15", "v_accvgpr_read_b32 v2, a15", "s_endpgm")) == []
+    # a product that the compiler issued itself is its own business
+    assert early_products(kernel(INLINE[1], "v_accvgpr_read_b32 v2, a15", "s_endpgm")) == []
+
+
+def test_every_source_with_such_assembly_is_checked():
+    read = re.compile(r'asm volatile\("[^"]*(ds_(read|load|bpermute)|v_mfma)')
     kernels = _build.CSRC / "kernels"
     headers = [h.name for h in kernels.glob("*.h") if read.search(h.read_text())]
     for src in sorted(kernels.glob("*.hip")):
